@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define TMX_ABI_VERSION 6
+#define TMX_ABI_VERSION 7
 /* int32 entries of tmx_index_t.scratch for a batch of `batch` requests and a capacity of R q-blocks */
 #define TMX_INDEX_SCRATCH_INTS(batch, R) ((batch) + 1 + 2 * ((R) + 1) + 8 * ((R) / 1024 + 1))
 
@@ -493,6 +493,74 @@ int tmx_gather_dequant_kv_fp8(const void* key_cache, const void* value_cache, in
                               const int32_t* cu_seqlens_k_dev, int32_t batch, int32_t max_seq_len,
                               int32_t num_kv_heads, int32_t head_dim, void* k_out, void* v_out, int32_t out_dtype,
                               float k_scale, float v_scale, void* stream);
+
+/* ------------------------------------------------------------------------
+ * 4-bit K/V cache (OCP MXFP4), kv_cache_dtype "mxfp4".  No counterpart in the reference, whose caches are 16-bit or
+ * fp8 (csrc/cache_kernels.cu:282-355): the same three operators -- write, read back, attention in place -- for a cache of
+ * 4.25 bits per value (3.76 times the tokens of a 16-bit cache in the same memory).
+ *
+ * Values: 32 neighbouring columns of a row share a power of two 2^e, stored as the byte e + 127; a value is one of 0,
+ * 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, times 2^e.  The write takes e = floor(log2(amax)) - 2, one more when amax >=
+ * 1.75 * 2^floor(log2(amax)), at least -126, and rounds x / 2^e to nearest, ties to the even code: nothing saturates.
+ * A block with an infinity or a NaN gets the byte 255 and reads back as NaN.
+ *
+ * Pages: a page of page_size tokens (a power of two, at least 16) of K or of V is num_kv_heads * page_size *
+ * (head_dim / 2 + head_dim / 32) bytes in one run, at page index * stride_page (bytes, a multiple of 16):
+ *   codes   K  [head][token][head_dim / 2]     two codes to a byte, the even column in the low half
+ *           V  [head][token / n][16][token % n][head_dim / 32]   with n = 512 / head_dim
+ *   scales     [head][head_dim / 32][token]
+ * head_dim 64 or 128.  Page numbers are checked on the device: a slot outside num_pages * page_size is skipped, keys
+ * whose block-table entry lies outside [0, num_pages) or past max_blocks count as NaN; nothing outside the cache is
+ * touched.
+ *
+ * tmx_reshape_and_cache_fp4: rows [num_tokens, num_kv_heads, head_dim] of bf16 / fp16 to flat slots (negative: skipped;
+ * the slots of a call are distinct).
+ * tmx_gather_dequant_kv_fp4: request b's key j to row cu_seqlens_k[b] + j of k_out / v_out [total_rows, num_kv_heads,
+ * head_dim] (rows outside are skipped): exact in bf16; in fp16 magnitudes past 65504 saturate there.  Prompts attend to
+ * these rows through tmx_attention in its contiguous mode.
+ * tmx_decode_attention_fp4: rows_per_request = m query rows per request, [batch * m, num_heads, head_dim]; row b m + j sits
+ * at position seq_lens[b] - m + j and attends to the keys up to its position (the keys of the step are in the cache
+ * already).  m = 1 is a decode step, m > 1 checks drafted tokens; m * num_heads / num_kv_heads <= 64.  seq_lens[b] <= 0
+ * marks padding, its out rows are left alone, as are rows at negative positions.  As in tmx_decode_attention the launch
+ * depends on the batch size alone (it replays under a graph) and the work area -- partial_o [rows][head_dim], partial_ml
+ * [rows][2], rows = tmx_decode_fp4_workspace_rows(...) -- belongs to one call at a time.
+ * ---------------------------------------------------------------------- */
+int tmx_reshape_and_cache_fp4(const void* key, const void* value, int64_t key_stride_t, int64_t key_stride_h,
+                              int64_t value_stride_t, int64_t value_stride_h, void* key_cache, void* value_cache,
+                              int64_t stride_page, int64_t num_pages, const int64_t* slot_mapping_dev, int32_t num_tokens,
+                              int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t in_dtype, void* stream);
+
+int tmx_gather_dequant_kv_fp4(const void* key_cache, const void* value_cache, int64_t stride_page, int64_t num_pages,
+                              const int32_t* block_table_dev, int64_t block_table_stride, int32_t max_blocks,
+                              int32_t page_size, const int32_t* seq_lens_dev, const int32_t* cu_seqlens_k_dev, int32_t batch,
+                              int32_t max_seq_len, int32_t num_kv_heads, int32_t head_dim, void* k_out, void* v_out,
+                              int64_t total_rows, int32_t out_dtype, void* stream);
+
+typedef struct tmx_decode_fp4_args_t {
+  uint32_t struct_size; /* sizeof(tmx_decode_fp4_args_t), ABI check */
+  int32_t io_dtype;     /* q element type: TMX_BF16 or TMX_F16 */
+  int32_t out_dtype;    /* == io_dtype, or TMX_F32 */
+  float scale;
+  int32_t batch, rows_per_request, num_heads, num_kv_heads, head_dim, page_size;
+  void* out;            /* (device) [batch * rows_per_request, num_heads, head_dim] */
+  int64_t out_stride_t, out_stride_h;
+  const void* q;        /* (device) the same shape */
+  int64_t q_stride_t, q_stride_h;
+  const void* k;        /* pages */
+  const void* v;
+  int64_t kv_stride_page, num_pages;
+  const int32_t* block_table; /* (device) [batch, block_table_stride] */
+  int64_t block_table_stride;
+  int32_t max_blocks;   /* entries of a row */
+  uint32_t flags;       /* 0 */
+  const int32_t* seq_lens; /* (device) [batch] */
+  float* partial_o;
+  float* partial_ml;
+  int64_t workspace_rows;
+} tmx_decode_fp4_args_t;
+
+int64_t tmx_decode_fp4_workspace_rows(int batch, int rows_per_request, int num_heads, int num_kv_heads, int head_dim, int num_cus);
+int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* args, void* stream);
 
 #ifdef __cplusplus
 }

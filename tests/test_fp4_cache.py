@@ -1,0 +1,469 @@
+"""The 4-bit (MXFP4) paged K/V cache: write, read-back and attention in place, against the format and the formulas in 64
+bits (tests/fp4_reference.py).  The write is exact, so it is compared byte for byte; attention outputs to a bound derived
+from their roundings (``fp4_reference.bound``)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import fp4_reference as ref
+from vllm_trianglemix_amd import _lib, ops
+
+gpu = pytest.mark.gpu
+DEV = "cuda:0"
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+
+
+# ------------------------------------------------------------------------------------------------ without a GPU
+def test_reference_format_round_trips():
+    rng = np.random.default_rng(0)
+    for dim in (64, 128):
+        for is_v in (False, True):
+            codes = rng.integers(0, 16, (3, 16, 2, dim)).astype(np.uint8)
+            scales = rng.integers(1, 254, (3, 16, 2, dim // 32)).astype(np.uint8)
+            raw = ref.pack(codes, scales, is_v)
+            assert raw.shape[1] == np.prod(ops.fp4_cache_shape(3, 16, 2, dim)[1:])
+            assert np.array_equal(ref.unpack(raw, 2, dim, 16, is_v), ref.values(codes, scales))
+    x = rng.standard_normal((5, 64)) * np.ldexp(1.0, rng.integers(-20, 20, (5, 1)))
+    c, s = ref.quantise(x)
+    y = ref.values(c, s)
+    # half a step of the top binade is 2^e, and amax >= 3.5 x 2^e
+    assert (np.abs(x - y).reshape(5, 2, 32) <= np.abs(x).reshape(5, 2, 32).max(-1, keepdims=True) / 3.5).all()
+    c2, s2 = ref.quantise(y)
+    assert np.array_equal(ref.values(c2, s2), y)  # its own values are fixed points
+
+
+def test_cache_shape_refusals():
+    assert ops.fp4_cache_shape(7, 32, 8, 128) == (7, 32, 8, 68)
+    for bad in ((4, 16, 8, 96), (4, 8, 8, 128), (4, 24, 8, 128)):
+        with pytest.raises(RuntimeError):
+            ops.fp4_cache_shape(*bad)
+
+
+def test_decode_struct_has_the_headers_size():
+    import os
+    import subprocess
+    import tempfile
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with tempfile.TemporaryDirectory() as d:
+        c, exe = os.path.join(d, "s.c"), os.path.join(d, "s")
+        with open(c, "w") as f:
+            f.write('#include <stdio.h>\n#include "trianglemix_hip.h"\nint main(void){printf("%zu", sizeof(tmx_decode_fp4_args_t));return 0;}\n')
+        subprocess.run(["gcc", "-I", os.path.join(root, "include"), c, "-o", exe], check=True)
+        assert int(subprocess.run([exe], check=True, capture_output=True, text=True).stdout) == ctypes.sizeof(_lib.DecodeFp4Args)
+
+
+def _args(**kw):
+    """A well-formed argument block over made-up, aligned addresses (calls with it are refused before any launch)."""
+    a = _lib.DecodeFp4Args()
+    a.struct_size, a.io_dtype, a.out_dtype, a.scale = ctypes.sizeof(a), _lib.TMX_BF16, _lib.TMX_BF16, 0.1
+    a.batch, a.rows_per_request, a.num_heads, a.num_kv_heads, a.head_dim, a.page_size = 2, 1, 8, 2, 128, 16
+    a.out = a.q = a.k = a.v = a.block_table = a.seq_lens = a.partial_o = a.partial_ml = 4096
+    a.out_stride_t = a.q_stride_t = 8 * 128
+    a.out_stride_h = a.q_stride_h = 128
+    a.kv_stride_page, a.num_pages, a.block_table_stride, a.max_blocks = 16 * 2 * 68, 9, 4, 4
+    a.workspace_rows = 1 << 40
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(struct_size=8), _lib.TMX_ERR_INVALID_ARG), (dict(io_dtype=_lib.TMX_F32), _lib.TMX_ERR_UNSUPPORTED),
+    (dict(out_dtype=_lib.TMX_F16), _lib.TMX_ERR_UNSUPPORTED), (dict(head_dim=96), _lib.TMX_ERR_UNSUPPORTED),
+    (dict(num_heads=7), _lib.TMX_ERR_INVALID_ARG), (dict(rows_per_request=0), _lib.TMX_ERR_INVALID_ARG),
+    (dict(rows_per_request=17), _lib.TMX_ERR_UNSUPPORTED), (dict(rows_per_request=2 ** 31 - 1), _lib.TMX_ERR_UNSUPPORTED),
+    (dict(scale=0.0), _lib.TMX_ERR_INVALID_ARG), (dict(scale=float("nan")), _lib.TMX_ERR_INVALID_ARG),
+    (dict(page_size=24), _lib.TMX_ERR_UNSUPPORTED), (dict(page_size=8), _lib.TMX_ERR_UNSUPPORTED),
+    (dict(q=None), _lib.TMX_ERR_INVALID_ARG), (dict(num_pages=0), _lib.TMX_ERR_INVALID_ARG),
+    (dict(kv_stride_page=16 * 2 * 68 - 16), _lib.TMX_ERR_INVALID_ARG), (dict(kv_stride_page=16 * 2 * 68 + 8), _lib.TMX_ERR_INVALID_ARG),
+    (dict(k=4104), _lib.TMX_ERR_INVALID_ARG), (dict(q_stride_h=132), _lib.TMX_ERR_INVALID_ARG),
+    (dict(max_blocks=-1), _lib.TMX_ERR_INVALID_ARG), (dict(batch=-1), _lib.TMX_ERR_INVALID_ARG),
+    (dict(batch=70000), _lib.TMX_ERR_UNSUPPORTED),
+])
+def test_decode_refuses_bad_arguments(change, code):
+    lib = _lib.load()
+    assert lib.tmx_decode_attention_fp4(ctypes.byref(_args(**change)), None) == code
+    assert lib.tmx_last_error()
+
+
+def test_decode_of_an_empty_batch_is_nothing():
+    assert _lib.load().tmx_decode_attention_fp4(ctypes.byref(_args(batch=0, q=None)), None) == _lib.TMX_OK
+    assert _lib.load().tmx_decode_attention_fp4(None, None) == _lib.TMX_ERR_INVALID_ARG
+    assert _lib.load().tmx_decode_fp4_workspace_rows(0, 1, 8, 2, 128, 256) == 0
+    assert _lib.load().tmx_decode_fp4_workspace_rows(3, 2, 8, 2, 128, 256) >= 3 * 2 * 8
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(dim=96), _lib.TMX_ERR_UNSUPPORTED), (dict(dtype=_lib.TMX_F32), _lib.TMX_ERR_UNSUPPORTED),
+    (dict(page=17), _lib.TMX_ERR_UNSUPPORTED), (dict(tokens=-1), _lib.TMX_ERR_INVALID_ARG), (dict(ptr=4104), _lib.TMX_ERR_INVALID_ARG),
+    (dict(stride=4), _lib.TMX_ERR_INVALID_ARG), (dict(page_stride=64), _lib.TMX_ERR_INVALID_ARG), (dict(ptr=None), _lib.TMX_ERR_INVALID_ARG),
+    (dict(heads=0), _lib.TMX_ERR_INVALID_ARG),
+])
+def test_write_and_gather_refuse_bad_arguments(change, code):
+    c = dict(dim=128, dtype=_lib.TMX_BF16, page=16, tokens=4, ptr=4096, stride=128, page_stride=16 * 2 * 68, heads=2, pages=9)
+    c.update(change)
+    lib = _lib.load()
+    assert lib.tmx_reshape_and_cache_fp4(c["ptr"], c["ptr"], c["stride"], c["stride"], c["stride"], c["stride"], c["ptr"],
+                                         c["ptr"], c["page_stride"], c["pages"], c["ptr"], c["tokens"], c["heads"], c["dim"],
+                                         c["page"], c["dtype"], None) == code
+    if "stride" in change:
+        return
+    assert lib.tmx_gather_dequant_kv_fp4(c["ptr"], c["ptr"], c["page_stride"], c["pages"], c["ptr"], 4, 4, c["page"], c["ptr"],
+                                         c["ptr"], 2, c["tokens"], c["heads"], c["dim"], c["ptr"], c["ptr"], 100, c["dtype"],
+                                         None) == code
+
+
+def test_tensors_on_the_cpu_are_refused():
+    k = torch.zeros(ops.fp4_cache_shape(4, 16, 2, 64), dtype=torch.uint8)
+    x = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        ops.reshape_and_cache_fp4(x, x, k, k, torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="HIP device"):
+        ops.gather_dequant_kv_fp4(k, k, torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, dtype=torch.int32),
+                                  torch.zeros(1, dtype=torch.int32), 1, 1, torch.bfloat16)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        ops.decode_attention_fp4(x, k, k, x, torch.zeros(3, 4, dtype=torch.int32), torch.ones(3, dtype=torch.int32), 1.0, (x, x))
+
+
+# ------------------------------------------------------------------------------------------------ on the GPU
+def _values_of(rng, shape, dtype):
+    """Rows over many magnitudes, with zeros, ties between codes and (fp16 / bf16) subnormals."""
+    x = rng.standard_normal(shape) * np.ldexp(1.0, rng.integers(-6, 7, (*shape[:-1], 1)))
+    x[rng.random(shape) < 0.05] = 0.0
+    grid = rng.choice(np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 6.99, 7.0]), shape)
+    x = np.where(rng.random(shape) < 0.2, grid, x)
+    x.reshape(-1, 32)[::7] = 0.0
+    x.reshape(-1, 32)[1::11] *= 2.0 ** (-24 if dtype == torch.float16 else -130)
+    if dtype == torch.float16:
+        x.reshape(-1, 32)[2::13] *= 2.0 ** 10
+        x = np.clip(x, -65504, 65504)
+    return torch.from_numpy(x).to(dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim, heads, page", [(128, 2, 16), (64, 3, 16), (128, 1, 64), (64, 8, 32), (128, 8, 16)])
+@pytest.mark.parametrize("tokens", [1, 5, 77])
+def test_write_stores_the_formats_bytes(dtype, dim, heads, page, tokens):
+    rng = np.random.default_rng(tokens * 1000 + dim + heads)
+    pages = -(-tokens // page) + 3
+    shape = ops.fp4_cache_shape(pages, page, heads, dim)
+    # rows as slices of a fused projection (a row stride of their own), K and V apart
+    qkv = torch.zeros(tokens, 3, heads, dim, dtype=dtype)
+    qkv[:, 1], qkv[:, 2] = _values_of(rng, (tokens, heads, dim), dtype), _values_of(rng, (tokens, heads, dim), dtype)
+    slots = rng.permutation(pages * page)[:tokens].astype(np.int64)
+    if tokens > 4:
+        slots[1], slots[3], slots[4] = -1, pages * page, 2 ** 62  # padding, and slots the cache does not have
+    start = rng.integers(0, 256, (2, *shape)).astype(np.uint8)
+    caches = [torch.from_numpy(s.copy()).to(DEV) for s in start]
+    d = qkv.to(DEV)
+    ops.reshape_and_cache_fp4(d[:, 1], d[:, 2], caches[0], caches[1], torch.from_numpy(slots).to(DEV))
+    for x in range(2):
+        rows = qkv[:, 1 + x].double().numpy()
+        want = start[x].reshape(pages, -1).copy()
+        full = np.zeros((pages, page, heads, dim), np.uint8), np.zeros((pages, page, heads, dim // 32), np.uint8)
+        mine = np.zeros((pages, page), bool)
+        codes, scales = ref.quantise(rows)
+        for t, s in enumerate(slots):
+            if 0 <= s < pages * page:
+                full[0][s // page, s % page], full[1][s // page, s % page] = codes[t], scales[t]
+                mine[s // page, s % page] = True
+        packed = ref.pack(*full, x == 1)
+        mask = ref.pack(np.where(mine[..., None, None], 15, 0).astype(np.uint8) + 0 * full[0],
+                        np.where(mine[..., None, None], 255, 0).astype(np.uint8) + 0 * full[1], x == 1)
+        want = (want & ~mask) | (packed & mask)
+        assert np.array_equal(caches[x].cpu().numpy().reshape(pages, -1), want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_blocks_with_infinities_and_nans_read_as_nan(dtype):
+    x = torch.ones(4, 1, 64, dtype=dtype)
+    x[0, 0, 3], x[1, 0, 40], x[2, 0, 0] = float("inf"), float("nan"), -float("inf")
+    caches = [torch.zeros(ops.fp4_cache_shape(1, 16, 1, 64), dtype=torch.uint8, device=DEV) for _ in range(2)]
+    ops.reshape_and_cache_fp4(x.to(DEV), x.to(DEV), *caches, torch.arange(4, device=DEV))
+    k, v = ops.gather_dequant_kv_fp4(*caches, torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.tensor([4], dtype=torch.int32, device=DEV),
+                                     torch.zeros(2, dtype=torch.int32, device=DEV), 4, 4, dtype)
+    for got in (k.cpu(), v.cpu()):
+        nan = torch.isnan(got[:, 0].float())
+        assert nan[0].tolist() == [True] * 32 + [False] * 32 and nan[1].tolist() == [False] * 32 + [True] * 32
+        assert nan[2].tolist() == [True] * 32 + [False] * 32 and not nan[3].any()
+        assert (got[:, 0][~nan] == 1).all()
+
+
+class Batch:
+    """Sequences of given lengths with scattered pages of a cache made of random rows (quantised on the host)."""
+
+    def __init__(self, seed, lens, heads, kv_heads, dim, page, m=1, spare=2, page_gap=0):
+        rng = np.random.default_rng(seed)
+        self.lens, self.H, self.Hkv, self.D, self.page, self.m = lens, heads, kv_heads, dim, page, m
+        need = [max(0, -(-n // page)) for n in lens]
+        pages = max(1, sum(need) + spare)
+        order = rng.permutation(pages)
+        self.table = np.full((len(lens), max(need + [1]) + 1), -1, np.int32)
+        at = 0
+        for b, c in enumerate(need):
+            self.table[b, :c] = order[at:at + c]
+            at += c
+        self.raw = []
+        for is_v in (False, True):
+            rows = rng.standard_normal((pages, page, kv_heads, dim))
+            rows[..., ::29] *= 4
+            self.raw.append(ref.pack(*ref.quantise(rows), is_v))
+        # a page stride of its own: the caches are views into a larger allocation
+        size = self.raw[0].shape[1]
+        self.caches = []
+        for raw in self.raw:
+            big = torch.full((pages, size + page_gap), 255, dtype=torch.uint8, device=DEV)
+            view = big.as_strided(ops.fp4_cache_shape(pages, page, kv_heads, dim),
+                                  (size + page_gap, size // page, size // page // kv_heads, 1))
+            view.copy_(torch.from_numpy(raw).to(DEV).view(view.shape))
+            self.caches.append(view)
+        self.q = rng.standard_normal((len(lens) * m, heads, dim))
+        self.bt = torch.from_numpy(self.table).to(DEV)
+        self.sl = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        self.scale = dim ** -0.5
+
+    def keys(self, b):
+        n = self.lens[b]
+        ids = self.table[b, :max(0, -(-n // self.page))]
+        return [ref.unpack(raw[ids], self.Hkv, self.D, self.page, x == 1).reshape(-1, self.Hkv, self.D)[:n] for x, raw in enumerate(self.raw)]
+
+    def run(self, dtype, out_dtype=None, fill=7.0):
+        q = torch.from_numpy(self.q).to(dtype)
+        out = torch.full(q.shape, fill, dtype=out_dtype or dtype, device=DEV)
+        ws = ops.decode_fp4_workspace(len(self.lens), self.m, self.H, self.Hkv, self.D, DEV)
+        ws[0].fill_(float("nan"))
+        ws[1].fill_(float("nan"))
+        ops.decode_attention_fp4(q.to(DEV), *self.caches, out, self.bt, self.sl, self.scale, ws, rows_per_request=self.m)
+        return q, out
+
+    def check(self, dtype, out_dtype=None):
+        q, out = self.run(dtype, out_dtype)
+        got, qd = out.double().cpu().numpy(), q.double().numpy()
+        for b, n in enumerate(self.lens):
+            rows = slice(b * self.m, (b + 1) * self.m)
+            if n <= 0:
+                assert (got[rows] == 7).all()
+                continue
+            o, av, qk = ref.attention(qd[rows], *self.keys(b), self.scale, self.m)
+            there = np.arange(self.m) >= self.m - n
+            assert (got[rows][~there] == 7).all()
+            lim = ref.bound(o, av, qk, n, self.D, HALF[out_dtype or dtype])[there]
+            err = np.abs(got[rows][there] - o[there])
+            assert (err <= lim).all(), (b, n, float((err / lim).max()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 32, 128])
+def test_decode_lengths(dtype, dim, page):
+    """Lengths around every boundary: one key, a 16-key half, a tile, a page, pieces that split."""
+    Batch(dim + page, [1, 2, 15, 16, 17, 31, 32, 33, 0, 63, 64, 65, 127, 129, 300, 1025, -3], 8, 2, dim, page).check(dtype)
+
+
+@gpu
+@pytest.mark.parametrize("heads, kv_heads", [(1, 1), (3, 1), (4, 4), (8, 1), (14, 2), (16, 1), (32, 8), (40, 2), (64, 1), (48, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_decode_head_layouts(heads, kv_heads, dtype):
+    Batch(heads * 10 + kv_heads, [700, 33, 0, 260], heads, kv_heads, 128, 16).check(dtype)
+    Batch(heads * 10 + kv_heads, [41, 514], heads, kv_heads, 64, 32).check(dtype, torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("m", [2, 3, 4, 8, 16])
+@pytest.mark.parametrize("dtype, dim", [(torch.bfloat16, 128), (torch.float16, 128), (torch.bfloat16, 64), (torch.float16, 64)])
+def test_several_rows_per_request(m, dtype, dim):
+    """Lengths below, at and above the number of rows; rows before the sequence's start are left alone."""
+    Batch(m, [m - 1, m, m + 1, 1, 0, 32, 33, 47, 64 + m, 500], 8, 2, dim, 16, m=m).check(dtype)
+
+
+@gpu
+def test_few_long_sequences_split_over_the_chip():
+    Batch(5, [20011], 8, 1, 128, 16).check(torch.bfloat16, torch.float32)
+    Batch(6, [9000, 1, 12345], 4, 1, 128, 64, m=2).check(torch.float16, torch.float32)
+
+
+@gpu
+def test_page_stride_and_query_strides():
+    b = Batch(8, [100, 45], 8, 2, 128, 16, page_gap=48)
+    b.check(torch.bfloat16)
+    # queries out of a fused projection, outputs into a wider row
+    q = torch.from_numpy(b.q).to(torch.bfloat16)
+    wide = torch.zeros(2, 20, 128, dtype=torch.bfloat16, device=DEV)
+    wide[:, 3:11] = q.to(DEV)
+    out = torch.full((2, 12, 128), 7.0, dtype=torch.bfloat16, device=DEV)
+    ws = ops.decode_fp4_workspace(2, 1, 8, 2, 128, DEV)
+    ops.decode_attention_fp4(wide[:, 3:11], *b.caches, out[:, 2:10], b.bt, b.sl, b.scale, ws)
+    _, want = b.run(torch.bfloat16)
+    assert torch.equal(out[:, 2:10], want) and (out[:, :2] == 7).all() and (out[:, 10:] == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_what_lies_behind_a_sequence_does_not_enter(dim):
+    """Keys past the sequence -- stale tokens of its last page, other rows' pages -- hold NaN scales."""
+    b = Batch(9, [37, 80], 8, 2, dim, 16)
+    _, want = b.run(torch.bfloat16)
+    for x, raw in enumerate(b.raw):
+        nb = b.Hkv * b.page * dim // 2
+        bad = raw.copy()
+        bad[b.table[0, 2], nb:].reshape(b.Hkv, dim // 32, b.page)[:, :, 5:] = 255
+        b.caches[x].copy_(torch.from_numpy(bad).to(DEV).view(b.caches[x].shape))
+    _, got = b.run(torch.bfloat16)
+    assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_nan_reaches_the_rows_that_see_it_and_no_other(dim, dtype):
+    """Drafted rows: a NaN block in V (or K) of a later position must not reach earlier rows."""
+    n, m, page = 45, 4, 16
+    for in_v in (False, True):
+        b = Batch(10, [n, 61], 8, 2, dim, page, m=m)
+        _, want = b.run(dtype)
+        nb = b.Hkv * page * dim // 2
+        key, head, block = n - 2, 1, 1  # seen by rows 2 and 3
+        raw = b.raw[in_v].copy()
+        raw[b.table[0, key // page], nb:].reshape(b.Hkv, dim // 32, page)[head, block, key % page] = 255
+        b.caches[in_v].copy_(torch.from_numpy(raw).to(DEV).view(b.caches[in_v].shape))
+        _, got = b.run(dtype)
+        nan = torch.isnan(got)
+        hit = torch.zeros_like(nan)
+        hit[2:4, 4:8, 32:64 if in_v else dim] = True
+        if not in_v:
+            hit[2:4, 4:8] = True
+        assert torch.equal(nan, hit)
+        assert torch.equal(got[~hit], want[~hit])
+
+
+@gpu
+def test_pages_that_do_not_exist_count_as_nan():
+    b = Batch(11, [40, 40, 90], 4, 1, 128, 16)
+    _, want = b.run(torch.bfloat16)
+    b.bt[0, 1] = 10 ** 6
+    b.bt[2, 0] = -5
+    q, got = b.run(torch.bfloat16)
+    assert torch.isnan(got[0]).all() and torch.isnan(got[2]).all() and torch.equal(got[1], want[1])
+    # a sequence longer than its row of the table
+    b.bt.copy_(torch.from_numpy(b.table))
+    out = torch.zeros_like(got)
+    ops.decode_attention_fp4(q.to(DEV), *b.caches, out, b.bt[:, :3], b.sl, b.scale, ops.decode_fp4_workspace(3, 1, 4, 1, 128, DEV))
+    assert torch.equal(out[:2], want[:2]) and torch.isnan(out[2]).all()
+    k, v = ops.gather_dequant_kv_fp4(*b.caches, b.bt[:, :3], b.sl, torch.tensor([0, 40, 80], dtype=torch.int32, device=DEV), 170, 90, torch.bfloat16)
+    assert torch.isnan(k[80 + 48:]).all() and torch.isnan(v[80 + 48:]).all() and not torch.isnan(k[:128]).any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim, heads, page", [(128, 2, 16), (64, 3, 32), (128, 8, 64), (64, 1, 16)])
+def test_gather_returns_the_values_the_cache_stands_for(dtype, dim, heads, page):
+    lens = [1, 0, 16, 33, 130]
+    b = Batch(12, lens, heads, heads, dim, page, page_gap=32)
+    cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    total = int(cu[-1])
+    out = [torch.full((total + 3, heads, dim), 7.0, dtype=dtype, device=DEV) for _ in range(2)]
+    got = ops.gather_dequant_kv_fp4(*b.caches, b.bt, b.sl, torch.from_numpy(cu).to(DEV), total, max(lens), dtype, out=out)
+    for x in range(2):
+        want = np.concatenate([b.keys(i)[x] for i in range(len(lens))])
+        assert np.array_equal(got[x][:total].double().cpu().numpy(), want)  # exact: one fraction bit
+        assert (got[x][total:] == 7).all()  # rows behind the last sequence
+    # fewer rows than the sequences have: the rest is skipped
+    out = [torch.full((total, heads, dim), 7.0, dtype=dtype, device=DEV) for _ in range(2)]
+    ops.gather_dequant_kv_fp4(*b.caches, b.bt, b.sl, torch.from_numpy(cu).to(DEV), 50, max(lens), dtype, out=out)
+    assert torch.equal(out[0][:50], got[0][:50]) and (out[0][50:] == 7).all()
+
+
+@gpu
+def test_fp16_rows_saturate():
+    x = torch.full((1, 1, 64), 65504.0, dtype=torch.float16, device=DEV)
+    x[0, 0, 1] = -65504.0
+    caches = [torch.zeros(ops.fp4_cache_shape(1, 16, 1, 64), dtype=torch.uint8, device=DEV) for _ in range(2)]
+    ops.reshape_and_cache_fp4(x, x, *caches, torch.zeros(1, dtype=torch.int64, device=DEV))
+    one, zero = torch.ones(1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    k, v = ops.gather_dequant_kv_fp4(*caches, zero.view(1, 1), one, zero, 1, 1, torch.float16)
+    assert torch.equal(k, x) and torch.equal(v, x)
+    k, v = ops.gather_dequant_kv_fp4(*caches, zero.view(1, 1), one, zero, 1, 1, torch.bfloat16)
+    assert k[0, 0, 0] == 65536 and v[0, 0, 1] == -65536
+
+
+@gpu
+def test_a_captured_step_replays_on_other_lengths():
+    b = Batch(13, [700, 40, 1], 8, 2, 128, 16)
+    q = torch.from_numpy(b.q).to(torch.bfloat16).to(DEV)
+    out = torch.zeros_like(q)
+    ws = ops.decode_fp4_workspace(3, 1, 8, 2, 128, DEV)
+    key = torch.randn(3, 2, 128, device=DEV).bfloat16()
+    slots = torch.full((3,), -1, dtype=torch.int64, device=DEV)
+
+    def step():
+        ops.reshape_and_cache_fp4(key, key, *b.caches, slots)
+        ops.decode_attention_fp4(q, *b.caches, out, b.bt, b.sl, b.scale, ws)
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for lens in ([700, 40, 1], [3, 0, 1], [650, 39, 1], [700, 40, 1]):
+        b.sl.copy_(torch.tensor(lens, dtype=torch.int32))
+        key.normal_()
+        q.normal_()
+        slots[0] = int(b.table[0, 0]) * 16 + 2
+        out.fill_(5.0)
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        out.fill_(5.0)
+        step()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out), lens
+
+
+@gpu
+def test_runs_on_the_callers_stream():
+    b = Batch(14, [900, 33], 8, 2, 128, 16)
+    _, want = b.run(torch.bfloat16)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        _, got = b.run(torch.bfloat16)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_refusals_on_the_gpu():
+    b = Batch(15, [20], 8, 2, 128, 16)
+    q = torch.zeros(1, 8, 128, dtype=torch.bfloat16, device=DEV)
+    ws = ops.decode_fp4_workspace(1, 1, 8, 2, 128, DEV)
+
+    def call(**kw):
+        a = dict(q=q, k=b.caches[0], v=b.caches[1], out=torch.zeros_like(q), bt=b.bt, sl=b.sl, ws=ws, m=1)
+        a.update(kw)
+        return ops.decode_attention_fp4(a["q"], a["k"], a["v"], a["out"], a["bt"], a["sl"], 0.1, a["ws"], rows_per_request=a["m"])
+
+    call()
+    for bad in (dict(q=q.float(), out=q.float()), dict(out=q.half()), dict(q=q[..., :64], out=q[..., :64]), dict(sl=b.sl.long()),
+                dict(bt=b.bt.long()), dict(bt=b.bt[0]), dict(ws=None), dict(ws=(ws[0][:8], ws[1])), dict(m=2), dict(m=0),
+                dict(k=b.caches[0].to(torch.int8)), dict(k=b.caches[0][..., :34]), dict(q=q[:, :7], out=q[:, :7]),
+                dict(k=b.caches[0].transpose(1, 2), v=b.caches[1].transpose(1, 2)), dict(sl=b.sl.cpu()), dict(ws=(ws[0].half(), ws[1]))):
+        with pytest.raises(RuntimeError):
+            call(**bad)
+    rows = torch.zeros(2, 2, 128, dtype=torch.bfloat16, device=DEV)
+    slots = torch.zeros(2, dtype=torch.int64, device=DEV)
+    ops.reshape_and_cache_fp4(rows, rows, *b.caches, slots[:0])
+    for bad in ((rows.float(), rows.float(), slots), (rows[:, :1], rows[:, :1], slots), (rows, rows[:1], slots), (rows, rows, slots.int()),
+                (rows[..., :64], rows[..., :64], slots), (rows, rows.half(), slots), (rows, rows, slots.cpu())):
+        with pytest.raises(RuntimeError):
+            ops.reshape_and_cache_fp4(bad[0], bad[1], *b.caches, bad[2])
+    cu = torch.tensor([0, 20], dtype=torch.int32, device=DEV)
+    for bad in (dict(dt=torch.float32), dict(bt=b.bt.long()), dict(sl=b.sl.long()), dict(out=(rows, rows))):
+        a = dict(dt=torch.bfloat16, bt=b.bt, sl=b.sl, out=None)
+        a.update(bad)
+        with pytest.raises(RuntimeError):
+            ops.gather_dequant_kv_fp4(*b.caches, a["bt"], a["sl"], cu, 20, 20, a["dt"], out=a["out"])

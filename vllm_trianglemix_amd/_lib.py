@@ -14,7 +14,7 @@ TMX_OK, TMX_ERR_INVALID_ARG, TMX_ERR_UNSUPPORTED, TMX_ERR_HIP, TMX_ERR_CAPACITY 
 TMX_F32, TMX_BF16, TMX_F16, TMX_FP8_E4M3 = range(4)
 TMX_MODE_NONE, TMX_MODE_CAUSAL, TMX_MODE_TRIANGLE = range(3)
 TMX_MASK_STREAMING, TMX_MASK_LAST, TMX_MASK_MIDDLE, TMX_MASK_TRIANGLE, TMX_MASK_DENSE = range(5)
-TMX_ABI_VERSION = 6
+TMX_ABI_VERSION = 7
 
 # every symbol include/trianglemix_hip.h declares
 EXPORTED_SYMBOLS = (
@@ -23,6 +23,7 @@ EXPORTED_SYMBOLS = (
     "tmx_reshape_and_cache_fp8", "tmx_gather_dequant_kv_fp8", "tmx_suggest_chunk_tiles",
     "tmx_attention_static_ws", "tmx_static_workspace_bytes", "tmx_static_workspace_warmup", "tmx_eager_attention_f32",
     "tmx_decode_attention", "tmx_decode_workspace_rows", "tmx_dense_stage_rows", "tmx_index_sizes_without_dense",
+    "tmx_reshape_and_cache_fp4", "tmx_gather_dequant_kv_fp4", "tmx_decode_attention_fp4", "tmx_decode_fp4_workspace_rows",
 )
 
 
@@ -93,6 +94,20 @@ class DecodeArgs(Structure):
     ]
 
 
+
+class DecodeFp4Args(Structure):
+    _fields_ = [
+        ("struct_size", c_uint32), ("io_dtype", c_int32), ("out_dtype", c_int32), ("scale", c_float),
+        ("batch", c_int32), ("rows_per_request", c_int32), ("num_heads", c_int32), ("num_kv_heads", c_int32),
+        ("head_dim", c_int32), ("page_size", c_int32),
+        ("out", c_void_p), ("out_stride_t", c_int64), ("out_stride_h", c_int64),
+        ("q", c_void_p), ("q_stride_t", c_int64), ("q_stride_h", c_int64),
+        ("k", c_void_p), ("v", c_void_p), ("kv_stride_page", c_int64), ("num_pages", c_int64),
+        ("block_table", c_void_p), ("block_table_stride", c_int64), ("max_blocks", c_int32), ("flags", c_uint32),
+        ("seq_lens", c_void_p), ("partial_o", c_void_p), ("partial_ml", c_void_p), ("workspace_rows", c_int64),
+    ]
+
+
 TMX_ATTN_SKIP_COMBINE, TMX_ATTN_ONLY_COMBINE, TMX_ATTN_SHORT_QUERIES, TMX_ATTN_NO_BAND, TMX_ATTN_NO_DENSE = 1, 2, 4, 8, 16
 TMX_ATTN_NO_DECODE, TMX_ATTN_DECODE_ONLY, TMX_ATTN_DECODE_VALU = 32, 64, 128
 TMX_DENSE_MIN_ROWS = 17  # query rows from which a request of a causal launch goes to the dense causal kernel
@@ -148,6 +163,14 @@ def load() -> ctypes.CDLL:
     lib.tmx_gather_dequant_kv_fp8.argtypes = [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32,
                                               c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                                               c_int32, c_float, c_float, c_void_p]
+    lib.tmx_reshape_and_cache_fp4.argtypes = [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                              c_int64, c_int64, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p]
+    lib.tmx_gather_dequant_kv_fp4.argtypes = [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int32, c_int32,
+                                              c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p,
+                                              c_int64, c_int32, c_void_p]
+    lib.tmx_decode_attention_fp4.argtypes = [POINTER(DecodeFp4Args), c_void_p]
+    lib.tmx_decode_fp4_workspace_rows.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int]
+    lib.tmx_decode_fp4_workspace_rows.restype = c_int64
     for name in EXPORTED_SYMBOLS:
         getattr(lib, name)  # AttributeError if a declared symbol is not exported
     if lib.tmx_abi_version() != TMX_ABI_VERSION:

@@ -780,3 +780,164 @@ def gather_dequant_kv_fp8(key_cache: torch.Tensor, value_cache: torch.Tensor, bl
             kc.shape[1], _ptr(seq_lens), _ptr(cu_seqlens_k), int(seq_lens.numel()), int(max_seq_len), hkv, d,
             _ptr(k_rows), _ptr(v_rows), dtype_code(out_dtype), float(k_scale), float(v_scale), _stream(kc.device)))
     return k_rows, v_rows
+
+
+# --------------------------------------------------------------------------- 4-bit (MXFP4) K/V cache
+FP4_BLOCK = 32  # columns that share a scale
+
+
+def fp4_cache_shape(num_blocks: int, page_size: int, num_kv_heads: int, head_dim: int):
+    """Shape of a K (or V) cache of uint8 in the 4-bit format: ``[num_blocks, page_size, Hkv, D / 2 + D / 32]``.  The
+    bytes of a page are one run in the library's own order (include/trianglemix_hip.h): codes of all heads, then their
+    scales -- the last three dimensions only count them."""
+    if head_dim not in (64, 128):
+        raise RuntimeError(f"a 4-bit cache has head size 64 or 128, not {head_dim}")
+    if page_size < 16 or page_size & (page_size - 1):
+        raise RuntimeError("page_size must be a power of two of at least 16")
+    return (num_blocks, page_size, num_kv_heads, head_dim // 2 + head_dim // FP4_BLOCK)
+
+
+def _fp4_caches(key_cache: torch.Tensor, value_cache: torch.Tensor) -> int:
+    """Checks a pair of 4-bit caches; the head size."""
+    _require_gpu(key_cache, "key_cache")
+    _require_gpu(value_cache, "value_cache")
+    if key_cache.dtype != torch.uint8 or value_cache.dtype != torch.uint8:
+        raise RuntimeError("a 4-bit cache is uint8 (ops.fp4_cache_shape)")
+    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape or key_cache.stride() != value_cache.stride():
+        raise RuntimeError("4-bit caches must be [num_blocks, page_size, Hkv, D / 2 + D / 32] with equal strides")
+    _, ps, hkv, width = key_cache.shape
+    if width not in (34, 68):
+        raise RuntimeError(f"a 4-bit cache's last dimension is D / 2 + D / 32 with D 64 or 128, not {width}")
+    if key_cache.device != value_cache.device or key_cache.stride()[1:] != (hkv * width, width, 1):
+        raise RuntimeError("a 4-bit page must be one run of bytes (only the page stride is free), both caches on one device")
+    return 64 if width == 34 else 128
+
+
+def _on(device: torch.device, *tensors) -> None:
+    for t, name in tensors:
+        _require_gpu(t, name)
+        if t.device != device:
+            raise RuntimeError(f"{name} is on {t.device}, the other tensors on {device}")
+
+
+def reshape_and_cache_fp4(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                          slot_mapping: torch.Tensor) -> None:
+    """Write this step's K/V rows ``[T, Hkv, D]`` (bf16 / fp16) into a 4-bit (MXFP4) paged cache: the counterpart of
+    ``reshape_and_cache`` and ``reshape_and_cache_fp8``.  32 neighbouring columns share a power of two, values round to
+    nearest (ties to the even code); a block with an infinity or a NaN reads back as NaN.  Slots that are negative or
+    past the cache are skipped; the others must be distinct."""
+    d = _fp4_caches(key_cache, value_cache)
+    dev = key_cache.device
+    _on(dev, (key, "key"), (value, "value"), (slot_mapping, "slot_mapping"))
+    if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1 or not slot_mapping.is_contiguous():
+        raise RuntimeError("slot_mapping must be contiguous int64")
+    if key.dim() != 3 or key.shape != value.shape or key.dtype != value.dtype or tuple(key.shape[1:]) != (key_cache.shape[2], d):
+        raise RuntimeError("key and value must be [T, Hkv, D] rows of one dtype that fit the cache")
+    n_tok = min(int(slot_mapping.numel()), key.shape[0])
+    if n_tok and (key.stride(2) != 1 or value.stride(2) != 1):
+        raise RuntimeError("the head dimension must be contiguous")
+    with torch.cuda.device(dev):
+        check(_lib.load().tmx_reshape_and_cache_fp4(
+            _ptr(key), _ptr(value), key.stride(0), key.stride(1), value.stride(0), value.stride(1), _ptr(key_cache),
+            _ptr(value_cache), key_cache.stride(0), key_cache.shape[0], _ptr(slot_mapping), n_tok, key.shape[1], d,
+            key_cache.shape[1], dtype_code(key.dtype), _stream(dev)))
+
+
+def gather_dequant_kv_fp4(key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor,
+                          seq_lens: torch.Tensor, cu_seqlens_k: torch.Tensor, total_rows: int, max_seq_len: int,
+                          out_dtype: torch.dtype, out: Optional[Sequence[torch.Tensor]] = None):
+    """The keys / values of every request of the step, out of a 4-bit cache, as contiguous 16-bit rows ``[total_rows,
+    Hkv, D]`` (request ``b``'s key ``j`` is row ``cu_seqlens_k[b] + j``), as ``gather_dequant_kv_fp8`` does for an fp8
+    cache.  Exact in bf16; in fp16 magnitudes past 65504 saturate there.  Rows past ``total_rows`` are skipped, keys whose
+    page does not exist are NaN.  Returns ``(k_rows, v_rows)``."""
+    d = _fp4_caches(key_cache, value_cache)
+    dev = key_cache.device
+    _on(dev, (block_table, "block_table"), (seq_lens, "seq_lens"), (cu_seqlens_k, "cu_seqlens_k"))
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+        raise RuntimeError("block_table must be int32 [B, max_blocks] with contiguous rows")
+    batch = int(seq_lens.numel())
+    if (seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous() or cu_seqlens_k.dtype != torch.int32
+            or not cu_seqlens_k.is_contiguous() or cu_seqlens_k.numel() < batch or block_table.shape[0] < batch):
+        raise RuntimeError("seq_lens and cu_seqlens_k must be contiguous int32, block_table must cover the batch")
+    if out_dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError("rows are read back as bfloat16 or float16")
+    hkv = key_cache.shape[2]
+    if out is None:
+        k_rows = torch.empty((max(total_rows, 1), hkv, d), dtype=out_dtype, device=dev)
+        v_rows = torch.empty_like(k_rows)
+    else:
+        k_rows, v_rows = out
+        _on(dev, (k_rows, "out[0]"), (v_rows, "out[1]"))
+        for x in (k_rows, v_rows):
+            if x.dim() != 3 or x.shape[0] < total_rows or tuple(x.shape[1:]) != (hkv, d) or not x.is_contiguous() or x.dtype != out_dtype:
+                raise RuntimeError("output rows must be contiguous [>= total_rows, Hkv, D] of out_dtype")
+    with torch.cuda.device(dev):
+        check(_lib.load().tmx_gather_dequant_kv_fp4(
+            _ptr(key_cache), _ptr(value_cache), key_cache.stride(0), key_cache.shape[0], _ptr(block_table),
+            block_table.stride(0), block_table.shape[1], key_cache.shape[1], _ptr(seq_lens), _ptr(cu_seqlens_k), batch,
+            int(max_seq_len), hkv, d, _ptr(k_rows), _ptr(v_rows), int(total_rows), dtype_code(out_dtype), _stream(dev)))
+    return k_rows, v_rows
+
+
+def decode_fp4_workspace(batch: int, rows_per_request: int, num_heads: int, num_kv_heads: int, head_dim: int, device):
+    """Work area of :func:`decode_attention_fp4` for a batch size (``tmx_decode_fp4_workspace_rows``).  Make it once and
+    keep it: a captured step replays with the same pointers.  One call at a time may use it."""
+    device = _device_of(device)
+    with torch.cuda.device(device):
+        rows = int(_lib.load().tmx_decode_fp4_workspace_rows(int(batch), int(rows_per_request), int(num_heads),
+                                                             int(num_kv_heads), int(head_dim), 0))
+    if rows < 0:
+        raise RuntimeError("tmx_decode_fp4_workspace_rows failed: " + _lib.load().tmx_last_error().decode("utf-8", "replace"))
+    rows = max(rows, 1)
+    return (torch.empty((rows * head_dim,), dtype=torch.float32, device=device),
+            torch.empty((rows * 2,), dtype=torch.float32, device=device))
+
+
+def decode_attention_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
+                         seq_lens: torch.Tensor, scale: float, workspace, rows_per_request: int = 1) -> torch.Tensor:
+    """Attention of a step of ``rows_per_request`` rows per request against a 4-bit (MXFP4) paged cache, read in place
+    (``tmx_decode_attention_fp4``).  Row ``b * rows_per_request + j`` of ``q`` ``[B * rows_per_request, H, D]`` sits at
+    position ``seq_lens[b] - rows_per_request + j`` and attends to the keys up to it; the step's own keys are in the cache
+    (``reshape_and_cache_fp4``).  One row is a decode step, several check drafted tokens (at most 64 rows per K/V head:
+    ``rows_per_request * H / Hkv <= 64``).  The launch depends on the batch size only: it can be captured and replayed
+    after ``seq_lens`` / ``block_table`` / the caches changed in place.  ``seq_lens[b] <= 0`` marks a padding request; its
+    rows of ``out``, and rows at negative positions, are left alone.  Keys whose page does not exist count as NaN.
+    ``workspace``: :func:`decode_fp4_workspace`."""
+    d = _fp4_caches(k, v)
+    dev = k.device
+    _on(dev, (q, "q"), (out, "out"), (block_table, "block_table"), (seq_lens, "seq_lens"))
+    if q.dim() != 3 or out.shape != q.shape or q.shape[2] != d:
+        raise RuntimeError("q and out must both be [B * rows_per_request, H, D] with the head size of the cache")
+    if q.numel() and (q.stride(2) != 1 or out.stride(2) != 1):
+        raise RuntimeError("the head dimension must be contiguous")
+    if out.dtype not in (q.dtype, torch.float32):
+        raise RuntimeError("out must have the dtype of q or be float32")
+    m = int(rows_per_request)
+    if m < 1 or q.shape[0] % m:
+        raise RuntimeError("q must hold rows_per_request rows for every request")
+    B, H = q.shape[0] // m, q.shape[1]
+    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.numel() < B or not seq_lens.is_contiguous():
+        raise RuntimeError("seq_lens must be contiguous int32 [B]")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.shape[0] < B:
+        raise RuntimeError("block_table must be int32 [B, max_blocks] with contiguous rows")
+    if workspace is None or len(workspace) < 2 or workspace[0] is None or workspace[1] is None:
+        raise RuntimeError("decode_attention_fp4 needs its work area (ops.decode_fp4_workspace for the batch size)")
+    part_o, part_ml = workspace[0], workspace[1]
+    _on(dev, (part_o, "workspace[0]"), (part_ml, "workspace[1]"))
+    if part_o.dtype != torch.float32 or part_ml.dtype != torch.float32 or not part_o.is_contiguous() or not part_ml.is_contiguous():
+        raise RuntimeError("the work area must be contiguous float32 (ops.decode_fp4_workspace)")
+    a = _lib.DecodeFp4Args()
+    a.struct_size = ctypes.sizeof(_lib.DecodeFp4Args)
+    a.io_dtype, a.out_dtype, a.scale = dtype_code(q.dtype), dtype_code(out.dtype), float(scale)
+    a.batch, a.rows_per_request, a.num_heads, a.num_kv_heads, a.head_dim, a.page_size = B, m, H, k.shape[2], d, k.shape[1]
+    a.out, a.out_stride_t, a.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
+    a.q, a.q_stride_t, a.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
+    a.k, a.v, a.kv_stride_page, a.num_pages = k.data_ptr(), v.data_ptr(), k.stride(0), k.shape[0]
+    a.block_table, a.block_table_stride, a.max_blocks = block_table.data_ptr(), block_table.stride(0), block_table.shape[1]
+    a.flags = 0
+    a.seq_lens = seq_lens.data_ptr()
+    a.partial_o, a.partial_ml = part_o.data_ptr(), part_ml.data_ptr()
+    a.workspace_rows = min(part_o.numel() // d, part_ml.numel() // 2)
+    with torch.cuda.device(dev):
+        check(_lib.load().tmx_decode_attention_fp4(ctypes.byref(a), _stream(dev)))
+    return out
