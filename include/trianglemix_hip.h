@@ -562,6 +562,41 @@ typedef struct tmx_decode_fp4_args_t {
 int64_t tmx_decode_fp4_workspace_rows(int batch, int rows_per_request, int num_heads, int num_kv_heads, int head_dim, int num_cus);
 int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Pages of a paged cache as units, whatever its type: a page is page_bytes bytes (a multiple of 16) at index * stride_page,
+ * `caches` the host array of the K and V caches of all layers (same sizes, num_pages pages each).  Which pages are in use
+ * follows from block_table [rows, cols] (int32, its rows block_table_stride apart) and seq_lens [rows]: row r holds its
+ * first ceil(seq_lens[r] / page_size) entries; a sequence is freed by a length of 0.  Entries that are no page numbers
+ * are passed over.  All lists are ascending or in a fixed order, never that of the workgroups.
+ *
+ * tmx_free_pages: free_out [num_pages] = the pages no row holds, ascending, -1 behind them; count_out[0] of them.
+ * tmx_plan_compaction: of the U pages in use, the k-th one at or past U is to go to the k-th free page before U:
+ * moves_out [num_pages / 2 + 1][2] = (from, to), totals_out = (U, number of moves), new_table [rows, cols] = the table
+ * afterwards (-1 past a row's entries).  The moves are then made by tmx_copy_pages with count = totals_out + 1.
+ * tmx_copy_pages: page pairs[k][0] to page pairs[k][1] (int32 or int64: pair_bits) in every cache, for k < num_pairs, and
+ * below *count if count (device) is given.  Pairs with a number outside the pool are skipped.  No page may be the target
+ * of two pairs, or of one and the source of another.  (The reference's copy_blocks, one layer at a time.)
+ * tmx_fork_pages: sequence i of `children` starts as row parents[i]: child_table[i] ([children, cols]) shares the parent's
+ * full pages; its partial last page, if it has one, is copied to page fresh[i] in every cache, which takes its place;
+ * -1 behind.  A parent outside the table gives a row of -1.  The fresh pages are distinct and not in use.
+ *
+ * work: tmx_pages_work_ints(rows, cols, num_pages) ints for the first two (0 for small tables: may be NULL).  Calls only
+ * enqueue; they can be captured.
+ * ---------------------------------------------------------------------- */
+int64_t tmx_pages_work_ints(int32_t rows, int32_t cols, int64_t num_pages);
+int tmx_free_pages(const int32_t* block_table_dev, int64_t block_table_stride, int32_t rows, int32_t cols,
+                   const int32_t* seq_lens_dev, int32_t page_size, int64_t num_pages, int32_t* free_out, int32_t* count_out,
+                   int32_t* work, int64_t work_ints, void* stream);
+int tmx_plan_compaction(const int32_t* block_table_dev, int64_t block_table_stride, int32_t rows, int32_t cols,
+                        const int32_t* seq_lens_dev, int32_t page_size, int64_t num_pages, int32_t* new_table,
+                        int32_t* moves_out, int32_t* totals_out, int32_t* work, int64_t work_ints, void* stream);
+int tmx_copy_pages(void* const* caches_host, int32_t num_caches, int64_t page_bytes, int64_t stride_page, int64_t num_pages,
+                   const void* pairs_dev, int32_t pair_bits, int32_t num_pairs, const int32_t* count_dev, void* stream);
+int tmx_fork_pages(void* const* caches_host, int32_t num_caches, int64_t page_bytes, int64_t stride_page, int64_t num_pages,
+                   const int32_t* block_table_dev, int64_t block_table_stride, int32_t rows, int32_t cols,
+                   const int32_t* seq_lens_dev, int32_t page_size, const int32_t* parents_dev, const int32_t* fresh_dev,
+                   int32_t children, int32_t* child_table, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,6 +24,7 @@ EXPORTED_SYMBOLS = (
     "tmx_attention_static_ws", "tmx_static_workspace_bytes", "tmx_static_workspace_warmup", "tmx_eager_attention_f32",
     "tmx_decode_attention", "tmx_decode_workspace_rows", "tmx_dense_stage_rows", "tmx_index_sizes_without_dense",
     "tmx_reshape_and_cache_fp4", "tmx_gather_dequant_kv_fp4", "tmx_decode_attention_fp4", "tmx_decode_fp4_workspace_rows",
+    "tmx_pages_work_ints", "tmx_free_pages", "tmx_plan_compaction", "tmx_copy_pages", "tmx_fork_pages",
 )
 
 
@@ -171,6 +172,15 @@ def load() -> ctypes.CDLL:
     lib.tmx_decode_attention_fp4.argtypes = [POINTER(DecodeFp4Args), c_void_p]
     lib.tmx_decode_fp4_workspace_rows.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int]
     lib.tmx_decode_fp4_workspace_rows.restype = c_int64
+    lib.tmx_pages_work_ints.argtypes = [c_int32, c_int32, c_int64]
+    lib.tmx_pages_work_ints.restype = c_int64
+    lib.tmx_free_pages.argtypes = [c_void_p, c_int64, c_int32, c_int32, c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p,
+                                   c_int64, c_void_p]
+    lib.tmx_plan_compaction.argtypes = [c_void_p, c_int64, c_int32, c_int32, c_void_p, c_int32, c_int64, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_int64, c_void_p]
+    lib.tmx_copy_pages.argtypes = [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int32, c_int32, c_void_p, c_void_p]
+    lib.tmx_fork_pages.argtypes = [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32, c_int32, c_void_p,
+                                   c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]
     for name in EXPORTED_SYMBOLS:
         getattr(lib, name)  # AttributeError if a declared symbol is not exported
     if lib.tmx_abi_version() != TMX_ABI_VERSION:

@@ -7,6 +7,7 @@
 //
 // Built as _trianglemix_C.so (plain C++, no device code) and loaded with
 // torch.ops.load_library(); the ops then live under torch.ops._trianglemix_C.
+#include <ATen/ops/empty.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
@@ -423,6 +424,232 @@ void gather_dequant_kv_fp8(Tensor& k_rows, Tensor& v_rows, const Tensor& key_cac
                                   (float)k_scale, (float)v_scale, stream_of(key_cache)));
 }
 
+// ---- 4-bit (MXFP4) cache ----
+void on_device(const Tensor& t, const Tensor& like, const char* name) {
+  TORCH_CHECK(t.device() == like.device(), "trianglemix: ", name, " is on ", t.device(), ", the other tensors on ", like.device());
+}
+
+// A pair of 4-bit caches [num_blocks, page_size, Hkv, D / 2 + D / 32]; the head size.
+int64_t fp4_caches(const Tensor& k, const Tensor& v) {
+  TORCH_CHECK(k.is_cuda(), "trianglemix: the caches must be on a HIP device");
+  TORCH_CHECK(k.scalar_type() == at::kByte && v.scalar_type() == at::kByte, "trianglemix: a 4-bit cache is uint8");
+  TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.strides() == v.strides(),
+              "trianglemix: 4-bit caches must be [num_blocks, page_size, Hkv, D / 2 + D / 32] with equal strides");
+  const int64_t width = k.size(3);
+  TORCH_CHECK(width == 34 || width == 68, "trianglemix: a 4-bit cache's last dimension is D / 2 + D / 32 with D 64 or 128, not ", width);
+  on_device(v, k, "value_cache");
+  TORCH_CHECK(k.stride(3) == 1 && k.stride(2) == width && k.stride(1) == k.size(2) * width,
+              "trianglemix: a 4-bit page must be one run of bytes (only the page stride is free)");
+  return width == 34 ? 64 : 128;
+}
+void table_rows(const Tensor& block_table, int64_t rows) {
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.stride(1) == 1 && block_table.size(0) >= rows,
+              "trianglemix: block_table must be int32 [B, max_blocks] with contiguous rows");
+}
+void lengths(const Tensor& t, int64_t n, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.numel() >= n, "trianglemix: ", name,
+              " must be contiguous int32 with an entry per request");
+}
+
+void reshape_and_cache_fp4(const Tensor& key, const Tensor& value, Tensor& key_cache, Tensor& value_cache, const Tensor& slot_mapping) {
+  const int64_t d = fp4_caches(key_cache, value_cache);
+  const DeviceGuard guard(key_cache.device());
+  on_device(key, key_cache, "key");
+  on_device(value, key_cache, "value");
+  on_device(slot_mapping, key_cache, "slot_mapping");
+  TORCH_CHECK(slot_mapping.scalar_type() == at::kLong && slot_mapping.dim() == 1 && slot_mapping.is_contiguous(),
+              "trianglemix: slot_mapping must be contiguous int64");
+  TORCH_CHECK(key.dim() == 3 && key.sizes() == value.sizes() && key.scalar_type() == value.scalar_type() &&
+                  key.size(1) == key_cache.size(2) && key.size(2) == d,
+              "trianglemix: key and value must be [T, Hkv, D] rows of one dtype that fit the cache");
+  const int64_t n = std::min<int64_t>(slot_mapping.numel(), key.size(0));
+  TORCH_CHECK(n == 0 || (key.stride(2) == 1 && value.stride(2) == 1), "trianglemix: the head dimension must be contiguous");
+  TORCH_CHECK(n <= 0x7fffffff, "trianglemix: too many rows");
+  check(tmx_reshape_and_cache_fp4(key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0), value.stride(1),
+                                  key_cache.data_ptr(), value_cache.data_ptr(), key_cache.stride(0), key_cache.size(0),
+                                  slot_mapping.data_ptr<int64_t>(), (int32_t)n, (int32_t)key.size(1), (int32_t)d,
+                                  (int32_t)key_cache.size(1), dtype_code(key), stream_of(key_cache)));
+}
+
+void gather_dequant_kv_fp4(Tensor& k_rows, Tensor& v_rows, const Tensor& key_cache, const Tensor& value_cache,
+                           const Tensor& block_table, const Tensor& seq_lens, const Tensor& cu_seqlens_k, int64_t total_rows,
+                           int64_t max_seq_len) {
+  const int64_t d = fp4_caches(key_cache, value_cache);
+  const DeviceGuard guard(key_cache.device());
+  for (const Tensor* t : {&k_rows, &v_rows}) {
+    on_device(*t, key_cache, "out");
+    TORCH_CHECK(t->dim() == 3 && t->size(0) >= total_rows && t->size(1) == key_cache.size(2) && t->size(2) == d && t->is_contiguous() &&
+                    t->scalar_type() == k_rows.scalar_type(),
+                "trianglemix: output rows must be contiguous [>= total_rows, Hkv, D] of one dtype");
+  }
+  on_device(block_table, key_cache, "block_table");
+  on_device(seq_lens, key_cache, "seq_lens");
+  on_device(cu_seqlens_k, key_cache, "cu_seqlens_k");
+  const int64_t batch = seq_lens.numel();
+  lengths(seq_lens, batch, "seq_lens");
+  lengths(cu_seqlens_k, batch, "cu_seqlens_k");
+  table_rows(block_table, batch);
+  TORCH_CHECK(max_seq_len <= 0x7fffffff && block_table.size(1) <= 0x7fffffff && batch <= 0x7fffffff, "trianglemix: sizes past 2^31");
+  check(tmx_gather_dequant_kv_fp4(key_cache.data_ptr(), value_cache.data_ptr(), key_cache.stride(0), key_cache.size(0),
+                                  block_table.data_ptr<int32_t>(), block_table.stride(0), (int32_t)block_table.size(1),
+                                  (int32_t)key_cache.size(1), seq_lens.data_ptr<int32_t>(), cu_seqlens_k.data_ptr<int32_t>(),
+                                  (int32_t)batch, (int32_t)max_seq_len, (int32_t)key_cache.size(2), (int32_t)d, k_rows.data_ptr(),
+                                  v_rows.data_ptr(), total_rows, dtype_code(k_rows), stream_of(key_cache)));
+}
+
+void decode_attention_fp4(Tensor& out, const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& block_table,
+                          const Tensor& seq_lens, Tensor& partial_o, Tensor& partial_ml, double scale, int64_t rows_per_request) {
+  const int64_t d = fp4_caches(key_cache, value_cache);
+  const DeviceGuard guard(key_cache.device());
+  on_device(query, key_cache, "q");
+  on_device(out, key_cache, "out");
+  on_device(block_table, key_cache, "block_table");
+  on_device(seq_lens, key_cache, "seq_lens");
+  on_device(partial_o, key_cache, "workspace");
+  on_device(partial_ml, key_cache, "workspace");
+  TORCH_CHECK(query.dim() == 3 && out.sizes() == query.sizes() && query.size(2) == d,
+              "trianglemix: q and out must both be [B * rows_per_request, H, D] with the head size of the cache");
+  TORCH_CHECK(query.numel() == 0 || (query.stride(2) == 1 && out.stride(2) == 1), "trianglemix: the head dimension must be contiguous");
+  TORCH_CHECK(out.scalar_type() == query.scalar_type() || out.scalar_type() == at::kFloat,
+              "trianglemix: out must have the dtype of q or be float32");
+  const int64_t m = rows_per_request;
+  TORCH_CHECK(m >= 1 && m <= 0x7fffffff && query.size(0) % m == 0, "trianglemix: q must hold rows_per_request rows for every request");
+  const int64_t batch = query.size(0) / m;
+  lengths(seq_lens, batch, "seq_lens");
+  table_rows(block_table, batch);
+  TORCH_CHECK(partial_o.scalar_type() == at::kFloat && partial_ml.scalar_type() == at::kFloat && partial_o.is_contiguous() &&
+                  partial_ml.is_contiguous(),
+              "trianglemix: the work area must be contiguous float32 (ops.decode_fp4_workspace)");
+  TORCH_CHECK(block_table.size(1) <= 0x7fffffff && batch <= 0x7fffffff, "trianglemix: sizes past 2^31");
+  tmx_decode_fp4_args_t a{};
+  a.struct_size = sizeof(a);
+  a.io_dtype = dtype_code(query);
+  a.out_dtype = dtype_code(out);
+  a.scale = (float)scale;
+  a.batch = (int32_t)batch;
+  a.rows_per_request = (int32_t)m;
+  a.num_heads = (int32_t)query.size(1);
+  a.num_kv_heads = (int32_t)key_cache.size(2);
+  a.head_dim = (int32_t)d;
+  a.page_size = (int32_t)key_cache.size(1);
+  a.out = out.data_ptr();
+  a.out_stride_t = out.stride(0);
+  a.out_stride_h = out.stride(1);
+  a.q = query.data_ptr();
+  a.q_stride_t = query.stride(0);
+  a.q_stride_h = query.stride(1);
+  a.k = key_cache.data_ptr();
+  a.v = value_cache.data_ptr();
+  a.kv_stride_page = key_cache.stride(0);
+  a.num_pages = key_cache.size(0);
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.block_table_stride = block_table.stride(0);
+  a.max_blocks = (int32_t)block_table.size(1);
+  a.seq_lens = seq_lens.data_ptr<int32_t>();
+  a.partial_o = partial_o.data_ptr<float>();
+  a.partial_ml = partial_ml.data_ptr<float>();
+  a.workspace_rows = std::min<int64_t>(partial_o.numel() / d, partial_ml.numel() / 2);
+  check(tmx_decode_attention_fp4(&a, stream_of(key_cache)));
+}
+
+// ---- pages ----
+struct PageList {
+  std::vector<void*> at;
+  int64_t bytes = 16, stride = 16, pages = 0;
+};
+PageList page_list(const std::vector<Tensor>& caches, const Tensor& like) {
+  PageList r;
+  TORCH_CHECK(like.is_cuda(), "trianglemix: page operators run on HIP devices only");
+  r.at.reserve(caches.size());
+  for (const Tensor& t : caches) {
+    const Tensor& f = caches[0];
+    TORCH_CHECK(t.device() == like.device(), "trianglemix: a cache is on ", t.device(), ", the other tensors on ", like.device());
+    TORCH_CHECK(t.dim() >= 2 && t.sizes() == f.sizes() && t.strides() == f.strides() && t.scalar_type() == f.scalar_type(),
+                "trianglemix: the caches must be [num_pages, ...] tensors of one shape, dtype and strides");
+    r.at.push_back(t.data_ptr());
+  }
+  if (!caches.empty()) {
+    const Tensor& f = caches[0];
+    int64_t run = 1;
+    for (int64_t i = f.dim() - 1; i >= 1; --i) {
+      TORCH_CHECK(f.size(i) == 1 || f.stride(i) == run, "trianglemix: a page must be one run of memory");
+      run *= f.size(i);
+    }
+    r.bytes = run * f.element_size();
+    r.pages = f.size(0);
+    r.stride = f.size(0) > 1 ? f.stride(0) * f.element_size() : r.bytes;
+  }
+  return r;
+}
+
+void copy_pages(const std::vector<Tensor>& caches, const Tensor& pairs) {
+  const PageList l = page_list(caches, pairs);
+  const DeviceGuard guard(pairs.device());
+  TORCH_CHECK((pairs.scalar_type() == at::kInt || pairs.scalar_type() == at::kLong) && pairs.dim() == 2 && pairs.size(1) == 2 &&
+                  pairs.is_contiguous() && pairs.size(0) <= 0x7fffffff,
+              "trianglemix: pairs must be contiguous int32 or int64 [n, 2]");
+  check(tmx_copy_pages(l.at.data(), (int32_t)l.at.size(), l.bytes, l.stride, l.pages, pairs.data_ptr(),
+                       pairs.scalar_type() == at::kInt ? 32 : 64, (int32_t)pairs.size(0), nullptr, stream_of(pairs)));
+}
+
+void page_table(const Tensor& block_table, const Tensor& seq_lens) {
+  table_rows(block_table, seq_lens.numel());
+  lengths(seq_lens, seq_lens.numel(), "seq_lens");
+  on_device(seq_lens, block_table, "seq_lens");
+  TORCH_CHECK(block_table.numel() <= 0x7fffffff, "trianglemix: the block table has more than 2^31 - 1 entries");
+}
+
+std::tuple<Tensor, Tensor> free_pages(const Tensor& block_table, const Tensor& seq_lens, int64_t num_pages, int64_t page_size) {
+  page_table(block_table, seq_lens);
+  const DeviceGuard guard(block_table.device());
+  TORCH_CHECK(num_pages >= 0 && num_pages <= (1 << 30) && page_size > 0 && page_size <= (1 << 30), "trianglemix: bad num_pages / page_size");
+  const int32_t rows = (int32_t)seq_lens.numel(), cols = (int32_t)block_table.size(1);
+  const int64_t work = tmx_pages_work_ints(rows, cols, num_pages);
+  Tensor buf = at::empty({num_pages + 1 + work}, block_table.options());
+  int32_t* b = buf.data_ptr<int32_t>();
+  check(tmx_free_pages(block_table.data_ptr<int32_t>(), block_table.stride(0), rows, cols, seq_lens.data_ptr<int32_t>(), (int32_t)page_size,
+                       num_pages, b, b + num_pages, b + num_pages + 1, work, stream_of(block_table)));
+  return {buf.narrow(0, 0, num_pages), buf.narrow(0, num_pages, 1)};
+}
+
+Tensor fork_pages(const std::vector<Tensor>& caches, const Tensor& block_table, const Tensor& seq_lens, const Tensor& parents,
+                  const Tensor& fresh, int64_t page_size) {
+  page_table(block_table, seq_lens);
+  const PageList l = page_list(caches, block_table);
+  const DeviceGuard guard(block_table.device());
+  lengths(parents, parents.numel(), "parents");
+  lengths(fresh, parents.numel(), "fresh");
+  on_device(parents, block_table, "parents");
+  on_device(fresh, block_table, "fresh");
+  TORCH_CHECK(page_size > 0 && page_size <= (1 << 30) && parents.numel() <= 0x7fffffff, "trianglemix: bad page_size or number of children");
+  Tensor child = at::empty({parents.numel(), block_table.size(1)}, block_table.options());
+  check(tmx_fork_pages(l.at.data(), (int32_t)l.at.size(), l.bytes, l.stride, l.pages, block_table.data_ptr<int32_t>(), block_table.stride(0),
+                       (int32_t)seq_lens.numel(), (int32_t)block_table.size(1), seq_lens.data_ptr<int32_t>(), (int32_t)page_size,
+                       parents.data_ptr<int32_t>(), fresh.data_ptr<int32_t>(), (int32_t)parents.numel(), child.data_ptr<int32_t>(),
+                       stream_of(block_table)));
+  return child;
+}
+
+std::tuple<Tensor, Tensor> compact_pages(const std::vector<Tensor>& caches, const Tensor& block_table, const Tensor& seq_lens,
+                                         int64_t page_size) {
+  page_table(block_table, seq_lens);
+  TORCH_CHECK(!caches.empty(), "trianglemix: compact_pages needs the caches (their first dimension is the pool)");
+  const PageList l = page_list(caches, block_table);
+  const DeviceGuard guard(block_table.device());
+  TORCH_CHECK(page_size > 0 && page_size <= (1 << 30) && l.pages <= (1 << 30), "trianglemix: bad page_size or number of pages");
+  const int32_t rows = (int32_t)seq_lens.numel(), cols = (int32_t)block_table.size(1);
+  const int64_t work = tmx_pages_work_ints(rows, cols, l.pages), moves = l.pages / 2 + 1;
+  Tensor buf = at::empty({2 * moves + 2 + work}, block_table.options());
+  Tensor table = at::empty({rows, cols}, block_table.options());
+  int32_t* b = buf.data_ptr<int32_t>();
+  check(tmx_plan_compaction(block_table.data_ptr<int32_t>(), block_table.stride(0), rows, cols, seq_lens.data_ptr<int32_t>(),
+                            (int32_t)page_size, l.pages, table.data_ptr<int32_t>(), b, b + 2 * moves, b + 2 * moves + 2, work,
+                            stream_of(block_table)));
+  check(tmx_copy_pages(l.at.data(), (int32_t)l.at.size(), l.bytes, l.stride, l.pages, b, 32, (int32_t)(l.pages / 2), b + 2 * moves + 1,
+                       stream_of(block_table)));
+  return {table, buf.narrow(0, 2 * moves, 1)};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(_trianglemix_C, m) {
@@ -459,6 +686,24 @@ TORCH_LIBRARY(_trianglemix_C, m) {
   m.def("trianglemix_gather_dequant_kv_fp8(Tensor! k_rows, Tensor! v_rows, Tensor key_cache, Tensor value_cache, "
         "Tensor block_table, Tensor seq_lens, Tensor cu_seqlens_k, int max_seq_len, float k_scale, float v_scale) -> ()");
   m.impl("trianglemix_gather_dequant_kv_fp8", c10::DispatchKey::CUDA, &gather_dequant_kv_fp8);
+  m.def("trianglemix_reshape_and_cache_fp4(Tensor key, Tensor value, Tensor! key_cache, Tensor! value_cache, "
+        "Tensor slot_mapping) -> ()");
+  m.impl("trianglemix_reshape_and_cache_fp4", c10::DispatchKey::CUDA, &reshape_and_cache_fp4);
+  m.def("trianglemix_gather_dequant_kv_fp4(Tensor! k_rows, Tensor! v_rows, Tensor key_cache, Tensor value_cache, "
+        "Tensor block_table, Tensor seq_lens, Tensor cu_seqlens_k, int total_rows, int max_seq_len) -> ()");
+  m.impl("trianglemix_gather_dequant_kv_fp4", c10::DispatchKey::CUDA, &gather_dequant_kv_fp4);
+  m.def("trianglemix_decode_attention_fp4(Tensor! out, Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_table, "
+        "Tensor seq_lens, Tensor! partial_o, Tensor! partial_ml, float scale, int rows_per_request=1) -> ()");
+  m.impl("trianglemix_decode_attention_fp4", c10::DispatchKey::CUDA, &decode_attention_fp4);
+  m.def("trianglemix_copy_pages(Tensor(a!)[] caches, Tensor pairs) -> ()");
+  m.impl("trianglemix_copy_pages", c10::DispatchKey::CUDA, &copy_pages);
+  m.def("trianglemix_free_pages(Tensor block_table, Tensor seq_lens, int num_pages, int page_size) -> (Tensor, Tensor)");
+  m.impl("trianglemix_free_pages", c10::DispatchKey::CUDA, &free_pages);
+  m.def("trianglemix_fork_pages(Tensor(a!)[] caches, Tensor block_table, Tensor seq_lens, Tensor parents, Tensor fresh, "
+        "int page_size) -> Tensor");
+  m.impl("trianglemix_fork_pages", c10::DispatchKey::CUDA, &fork_pages);
+  m.def("trianglemix_compact_pages(Tensor(a!)[] caches, Tensor block_table, Tensor seq_lens, int page_size) -> (Tensor, Tensor)");
+  m.impl("trianglemix_compact_pages", c10::DispatchKey::CUDA, &compact_pages);
 }
 
 // The extension is also a Python module, so that a plain `import` of the shared object runs the

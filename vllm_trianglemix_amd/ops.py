@@ -813,6 +813,14 @@ def _fp4_caches(key_cache: torch.Tensor, value_cache: torch.Tensor) -> int:
     return 64 if width == 34 else 128
 
 
+def _call(op, *args):
+    """A registered operator's call: its refusals come as TmxError, like the library's own."""
+    try:
+        return op(*args)
+    except (RuntimeError, NotImplementedError) as e:
+        raise _lib.TmxError(-1, str(e)) from None
+
+
 def _on(device: torch.device, *tensors) -> None:
     for t, name in tensors:
         _require_gpu(t, name)
@@ -826,6 +834,11 @@ def reshape_and_cache_fp4(key: torch.Tensor, value: torch.Tensor, key_cache: tor
     ``reshape_and_cache`` and ``reshape_and_cache_fp8``.  32 neighbouring columns share a power of two, values round to
     nearest (ties to the even code); a block with an infinity or a NaN reads back as NaN.  Slots that are negative or
     past the cache are skipped; the others must be distinct."""
+    _require_gpu(key_cache, "key_cache")
+    C = _op_binding()
+    if C is not None:
+        _call(C.trianglemix_reshape_and_cache_fp4, key, value, key_cache, value_cache, slot_mapping)
+        return
     d = _fp4_caches(key_cache, value_cache)
     dev = key_cache.device
     _on(dev, (key, "key"), (value, "value"), (slot_mapping, "slot_mapping"))
@@ -850,6 +863,19 @@ def gather_dequant_kv_fp4(key_cache: torch.Tensor, value_cache: torch.Tensor, bl
     Hkv, D]`` (request ``b``'s key ``j`` is row ``cu_seqlens_k[b] + j``), as ``gather_dequant_kv_fp8`` does for an fp8
     cache.  Exact in bf16; in fp16 magnitudes past 65504 saturate there.  Rows past ``total_rows`` are skipped, keys whose
     page does not exist are NaN.  Returns ``(k_rows, v_rows)``."""
+    _require_gpu(key_cache, "key_cache")
+    C = _op_binding()
+    if C is not None:
+        if out is None:
+            d = 64 if key_cache.shape[-1] == 34 else 128
+            shape = (max(int(total_rows), 1), key_cache.shape[-2], d)
+            out = [torch.empty(shape, dtype=out_dtype, device=key_cache.device) for _ in range(2)]
+        k_rows, v_rows = out
+        if k_rows.dtype != out_dtype:
+            raise RuntimeError("output rows must be contiguous [>= total_rows, Hkv, D] of out_dtype")
+        _call(C.trianglemix_gather_dequant_kv_fp4, k_rows, v_rows, key_cache, value_cache, block_table, seq_lens, cu_seqlens_k,
+              int(total_rows), int(max_seq_len))
+        return k_rows, v_rows
     d = _fp4_caches(key_cache, value_cache)
     dev = key_cache.device
     _on(dev, (block_table, "block_table"), (seq_lens, "seq_lens"), (cu_seqlens_k, "cu_seqlens_k"))
@@ -903,6 +929,14 @@ def decode_attention_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out:
     after ``seq_lens`` / ``block_table`` / the caches changed in place.  ``seq_lens[b] <= 0`` marks a padding request; its
     rows of ``out``, and rows at negative positions, are left alone.  Keys whose page does not exist count as NaN.
     ``workspace``: :func:`decode_fp4_workspace`."""
+    if workspace is None or len(workspace) < 2 or workspace[0] is None or workspace[1] is None:
+        raise RuntimeError("decode_attention_fp4 needs its work area (ops.decode_fp4_workspace for the batch size)")
+    _require_gpu(k, "k")
+    C = _op_binding()
+    if C is not None:
+        _call(C.trianglemix_decode_attention_fp4, out, q, k, v, block_table, seq_lens, workspace[0], workspace[1], float(scale),
+              int(rows_per_request))
+        return out
     d = _fp4_caches(k, v)
     dev = k.device
     _on(dev, (q, "q"), (out, "out"), (block_table, "block_table"), (seq_lens, "seq_lens"))
@@ -920,8 +954,6 @@ def decode_attention_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out:
         raise RuntimeError("seq_lens must be contiguous int32 [B]")
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.shape[0] < B:
         raise RuntimeError("block_table must be int32 [B, max_blocks] with contiguous rows")
-    if workspace is None or len(workspace) < 2 or workspace[0] is None or workspace[1] is None:
-        raise RuntimeError("decode_attention_fp4 needs its work area (ops.decode_fp4_workspace for the batch size)")
     part_o, part_ml = workspace[0], workspace[1]
     _on(dev, (part_o, "workspace[0]"), (part_ml, "workspace[1]"))
     if part_o.dtype != torch.float32 or part_ml.dtype != torch.float32 or not part_o.is_contiguous() or not part_ml.is_contiguous():
@@ -941,3 +973,129 @@ def decode_attention_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out:
     with torch.cuda.device(dev):
         check(_lib.load().tmx_decode_attention_fp4(ctypes.byref(a), _stream(dev)))
     return out
+
+
+# --------------------------------------------------------------------------- pages of a cache
+def _page_list(caches: Sequence[torch.Tensor], device: torch.device):
+    """(addresses, bytes of a page, bytes from page to page, pages) of caches ``[num_pages, ...]``."""
+    first = caches[0] if len(caches) else None
+    for t in caches:
+        _on(device, (t, "a cache"))
+        if t.dim() < 2 or t.shape != first.shape or t.stride() != first.stride() or t.dtype != first.dtype:
+            raise RuntimeError("the caches must be [num_pages, ...] tensors of one shape, dtype and strides")
+    if first is None:
+        return (ctypes.c_void_p * 1)(), 16, 16, 0
+    run = 1
+    for n, s in zip(reversed(first.shape[1:]), reversed(first.stride()[1:])):
+        if n != 1 and s != run:
+            raise RuntimeError("a page must be one run of memory")
+        run *= n
+    size = run * first.element_size()
+    stride = first.stride(0) * first.element_size() if first.shape[0] > 1 else size
+    return (ctypes.c_void_p * len(caches))(*[t.data_ptr() for t in caches]), size, stride, first.shape[0]
+
+
+def _page_table(block_table: torch.Tensor, seq_lens: torch.Tensor) -> torch.device:
+    _require_gpu(block_table, "block_table")
+    _on(block_table.device, (seq_lens, "seq_lens"))
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1
+            or block_table.shape[0] < seq_lens.numel()):
+        raise RuntimeError("block_table must be int32 [rows, max_blocks] with contiguous rows")
+    _page_ints(seq_lens, seq_lens.numel(), "seq_lens")
+    return block_table.device
+
+
+def _page_ints(t: torch.Tensor, n: int, name: str) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() < n:
+        raise RuntimeError(f"{name} must be contiguous int32 with an entry per row")
+
+
+def copy_pages(caches: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
+    """Page ``pairs[k, 0]`` to page ``pairs[k, 1]`` (int32 or int64 ``[n, 2]`` on the device) in every cache of the list,
+    in one launch (the reference's ``copy_blocks``).  ``caches``: ``[num_pages, ...]`` tensors of one shape and dtype,
+    any cache type, usually the K and V caches of all layers.  Pairs with a number outside the pool are skipped; no page
+    may be the target of two pairs, or of one and the source of another."""
+    _require_gpu(pairs, "pairs")
+    C = _op_binding()
+    if C is not None:
+        _call(C.trianglemix_copy_pages, caches, pairs)
+        return
+    dev = pairs.device
+    at, size, stride, pages = _page_list(caches, dev)
+    if pairs.dtype not in (torch.int32, torch.int64) or pairs.dim() != 2 or pairs.shape[1] != 2 or not pairs.is_contiguous():
+        raise RuntimeError("pairs must be contiguous int32 or int64 [n, 2]")
+    with torch.cuda.device(dev):
+        check(_lib.load().tmx_copy_pages(at, len(caches), size, stride, pages, _ptr(pairs), 8 * pairs.element_size(), pairs.shape[0],
+                                         None, _stream(dev)))
+
+
+def free_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, num_pages: int, page_size: int):
+    """The pages of a pool of ``num_pages`` that no sequence uses: ``(ids, count)``, int32 ``[num_pages]`` ascending with -1
+    behind the last, and ``[1]``.  Row ``r`` of ``block_table`` uses its first ``ceil(seq_lens[r] / page_size)`` entries; a
+    sequence is freed by a length of 0.  Nothing is read back to the host."""
+    _require_gpu(block_table, "block_table")
+    C = _op_binding()
+    if C is not None:
+        return _call(C.trianglemix_free_pages, block_table, seq_lens, int(num_pages), int(page_size))
+    dev = _page_table(block_table, seq_lens)
+    if num_pages < 0:
+        raise RuntimeError("num_pages must not be negative")
+    rows, cols = seq_lens.numel(), block_table.shape[1]
+    lib = _lib.load()
+    work = lib.tmx_pages_work_ints(rows, cols, num_pages)
+    buf = torch.empty((num_pages + 1 + work,), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        check(lib.tmx_free_pages(_ptr(block_table), block_table.stride(0), rows, cols, _ptr(seq_lens), int(page_size), int(num_pages),
+                                 buf.data_ptr(), buf[num_pages:].data_ptr(), buf[num_pages + 1:].data_ptr(), work, _stream(dev)))
+    return buf[:num_pages], buf[num_pages:num_pages + 1]
+
+
+def fork_pages(caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor,
+               fresh: torch.Tensor, page_size: int) -> torch.Tensor:
+    """Sequences that start as copies of running ones (parallel samples, beams): row ``i`` of the returned int32 ``[n,
+    max_blocks]`` table shares the full pages of row ``parents[i]``; the parent's partial last page, if it has one, is
+    copied to page ``fresh[i]`` in every cache of the list and that page takes its place.  Entries behind are -1; a parent
+    that is no row gives a row of -1.  The fresh pages (:func:`free_pages`) are distinct and not in use; one whose parent
+    ends on a page boundary stays free."""
+    _require_gpu(block_table, "block_table")
+    C = _op_binding()
+    if C is not None:
+        return _call(C.trianglemix_fork_pages, caches, block_table, seq_lens, parents, fresh, int(page_size))
+    dev = _page_table(block_table, seq_lens)
+    at, size, stride, pages = _page_list(caches, dev)
+    _on(dev, (parents, "parents"), (fresh, "fresh"))
+    n = parents.numel()
+    _page_ints(parents, n, "parents")
+    _page_ints(fresh, n, "fresh")
+    child = torch.empty((n, block_table.shape[1]), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        check(_lib.load().tmx_fork_pages(at, len(caches), size, stride, pages, _ptr(block_table), block_table.stride(0), seq_lens.numel(),
+                                         block_table.shape[1], _ptr(seq_lens), int(page_size), _ptr(parents), _ptr(fresh), n, _ptr(child),
+                                         _stream(dev)))
+    return child
+
+
+def compact_pages(caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq_lens: torch.Tensor, page_size: int):
+    """Closes a pool up: afterwards its ``U`` pages in use are the pages 0 .. U - 1.  Of the pages in use the k-th one at or
+    past U moves to the k-th free page before it, in every cache of the list.  Returns ``(table, count)``: the block table
+    afterwards (a new int32 ``[rows, max_blocks]``, -1 behind a row's entries) and U (int32 ``[1]``).  Pages shared by
+    several rows move once.  Nothing is read back to the host."""
+    _require_gpu(block_table, "block_table")
+    C = _op_binding()
+    if C is not None:
+        return _call(C.trianglemix_compact_pages, caches, block_table, seq_lens, int(page_size))
+    dev = _page_table(block_table, seq_lens)
+    if not len(caches):
+        raise RuntimeError("compact_pages needs the caches (their first dimension is the pool)")
+    at, size, stride, pages = _page_list(caches, dev)
+    rows, cols = seq_lens.numel(), block_table.shape[1]
+    lib = _lib.load()
+    work, moves = lib.tmx_pages_work_ints(rows, cols, pages), pages // 2 + 1
+    buf = torch.empty((2 * moves + 2 + work,), dtype=torch.int32, device=dev)
+    table = torch.empty((rows, cols), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        b = buf.data_ptr()
+        check(lib.tmx_plan_compaction(_ptr(block_table), block_table.stride(0), rows, cols, _ptr(seq_lens), int(page_size), pages,
+                                      _ptr(table), b, b + 8 * moves, b + 8 * moves + 8, work, _stream(dev)))
+        check(lib.tmx_copy_pages(at, len(caches), size, stride, pages, b, 32, pages // 2, b + 8 * moves + 4, _stream(dev)))
+    return table, buf[2 * moves:2 * moves + 1]
