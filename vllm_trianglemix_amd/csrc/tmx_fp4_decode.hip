@@ -1,28 +1,29 @@
 // Attention of a step's query rows against a 4-bit (MXFP4) paged K/V cache, for gfx950 (MI355X): one row per request
 // (decode) or the last few positions of each (drafted tokens checked in one step).  Such a step reads all of its K/V
-// once and multiplies little, so it is bound by the bytes of the cache; the 4-bit codes become bf16 in registers, which is
-// exact (a code has one fraction bit, the scale is a power of two), and both products run on the matrix cores.
+// once and multiplies little, so it is bound by the bytes of the cache; what the kernel has to do is ask for them in whole
+// lines, early, and keep the vector units out of their way.
 //
-//   workgroup = 4 waves = one piece of a request's keys x one K/V head; the waves take the piece's 32-key tiles in turn
-//   and meet only at the end.  Rows = rows_per_request x (query heads per K/V head), all of them columns of the same
-//   products, so a head's K/V are read once whatever the group size.
-//   Scores S^T = K Q^T (v_mfma_f32_16x16x32_bf16, 2 x D / 32 of them): lane (m = lane % 16, g = lane / 16) holds key row m
-//   and columns [g D/4, (g + 1) D/4) of it, one 16-byte load and one scale for D = 128; the head dimension may be summed
-//   in any order as long as Q^T is laid out alike.  Row m of the first / second product is key 8 (m / 4) + (m % 4), + 4
-//   for the second: a lane's 8 scores are then the keys 8 g .. 8 g + 7, exactly the ones it has to hold as operand of
-//   the second product, and the probabilities never leave their lane.
-//   Output O^T = V^T P^T: lane (m, g) needs columns [m D/16, (m + 1) D/16) of keys 8 g .. + 7.  The cache keeps V in that
-//   order (tmx_fp4.h): one or two 16-byte loads, 32 conversions and 32 byte permutes turn them into operands.  No LDS.
+//   workgroup = 4 waves = a span of 32-key tiles x one K/V head; the waves take the span's tiles in turn and meet only at
+//   a request's end.  Rows = rows_per_request x (query heads per K/V head), all of them columns of the same products, so
+//   a head's K/V are read once whatever the group size.
+//   Scores S^T = K Q^T: K goes to the matrix cores as it lies in the cache (v_mfma_scale_f32_16x16x128_f8f6f4, 4-bit
+//   operand, one scale byte per key and 32 columns), nothing is converted.  Q^T is the 8-bit operand, split into two terms
+//   of 4 significant bits (bf16 queries: 8 bits) or three (fp16: 11), each with a power of two per 32 columns: the terms
+//   hold every query value down to 2^-14 of its block's largest exactly and smaller ones to 2^-22 (bf16; fp16 2^-26) of it,
+//   below the rounding of the fp32 sums.  Row m of product t is key 16 t + m of the tile.
+//   Output O^T = V^T P^T (v_mfma_f32_16x16x32_bf16): lane (m = lane % 16, g = lane / 16) needs columns [m D/16, (m + 1)
+//   D/16) of the 8 keys whose scores it holds, 4 g .. 4 g + 3 and 16 + 4 g .. + 3.  The cache keeps V in that order
+//   (tmx_fp4.h), so V comes straight from memory, becomes bf16 (exact: one fraction bit, power-of-two scales) by 32
+//   conversions and is paired by 32 byte permutes; the probabilities never leave their lane.  No LDS in the loop.
 //   Probabilities are held as two bf16 terms (16 significant bits; one term alone would cost as much accuracy as the
 //   rounding of the output).  Up to 8 rows, columns 8..15 repeat the rows and carry the second term: no extra product.
-//   fp16 queries are split into two bf16 terms as well (exact: 11 bits in 8 + 8).
+//   Their sum is one more product, with ones.
+//   Every load instruction of the loop reads one contiguous run of a page-half (1 KB of codes) from a scalar base.
 //   The running maximum is raised only when a score exceeds it by more than 2^kSlack (factors stay below 2^8 in fp32).
-//   A piece's result goes to the output row, or to partial results that a second launch joins.
 #include <atomic>
 #include <type_traits>
 
 #include "tmx_common.h"
-#include "tmx_decode_plan.h"
 #include "tmx_fp4.h"
 
 namespace tmx {
@@ -30,6 +31,9 @@ namespace tmx {
 typedef __attribute__((ext_vector_type(4))) float f4_f32x4;
 typedef __attribute__((ext_vector_type(8))) __bf16 f4_bf16x8;
 typedef __attribute__((ext_vector_type(2))) float f4_f32x2;
+typedef __attribute__((ext_vector_type(8))) int f4_i32x8;
+typedef __attribute__((ext_vector_type(2))) unsigned short f4_u16x2;
+typedef __attribute__((ext_vector_type(2))) short f4_s16x2;
 
 constexpr float kFp4MinusBig = -3.0e38f;  // below every finite score, and finite
 constexpr float kFp4Slack = 8.0f;
@@ -46,12 +50,15 @@ struct Fp4DecodeParams {
   int max_blocks, page_shift;
   const int32_t* seq_lens;
   int batch, m, H, Hkv, G;
+  int len_cap;  // keys the block table has room for, + m: longer sequences read as this long (and as NaN)
   int64_t q_stride_t, q_stride_h, out_stride_t, out_stride_h;  // elements
   int out_f32;
   float scale_log2;
-  float* partial_o;   // [piece][row of the request][head][D]
-  float* partial_ml;  // [piece][row of the request][head][2]
-  int plan_slots;
+  float* partial_o;   // [slot][row of the request][head][D]
+  float* partial_ml;  // [slot][row of the request][head][2]
+  int spans;       // workgroups per unit
+  int row_groups;  // groups of 32 rows of a K/V head, each with workgroups of its own
+  int units;       // K/V heads x row groups
 };
 
 template <typename T>
@@ -73,425 +80,615 @@ __device__ __forceinline__ void fp4_store_out(void* out, int64_t at, float x, bo
   else reinterpret_cast<_Float16*>(out)[at] = (_Float16)x;
 }
 
-// Workgroups resident per CU by the registers that the accumulators of `rows` rows leave.
-constexpr int fp4_wgs_per_cu(int head_dim, int rows) { return rows <= 16 ? (head_dim == 128 ? 3 : 4) : (rows <= 32 ? 2 : 1); }
+// ---- the plan: the 32-key tiles of all requests, one after the other, are cut into equal spans, one per workgroup and
+// K/V head, whatever the requests' lengths are.  A request's beginning counts as kFp4Begin tiles more: what it costs to
+// change over (queries split anew, the waves' sums joined and written).  A span may begin and end inside requests: piece
+// (span w, request b) of a request that lies in several spans leaves its result in slot w + b -- both only grow along the
+// tiles, so no two pieces share a slot -- and the pieces are joined afterwards.  Every wave works the plan out for itself, without a barrier: lane l
+// counts the tiles of a run of requests, six shuffles sum the lanes. ----
+constexpr int kFp4MinSpan = 4;  // a tile per wave
+constexpr int kFp4Begin = 12;
+__device__ __forceinline__ int fp4_len(const Fp4DecodeParams& p, int n) { return imin(n, p.len_cap); }
+__device__ __forceinline__ int fp4_tiles(int n) { return n > 0 ? (n + kBlockN - 1) / kBlockN : 0; }
+__device__ __forceinline__ int fp4_cost(int n) { return n > 0 ? fp4_tiles(n) + kFp4Begin : 0; }
+__device__ __forceinline__ int fp4_span(int tiles, int spans) {
+  const int c = ((tiles + spans - 1) / spans + 3) & ~3;
+  return imax(c, kFp4MinSpan);
+}
+struct Fp4Plan {
+  int per;                  // requests per lane
+  int mine, before, total;  // cost of this lane's requests, of those before them, of all
+};
+__device__ __forceinline__ Fp4Plan fp4_plan(const Fp4DecodeParams& p, int lane) {
+  Fp4Plan r;
+  r.per = (p.batch + 63) >> 6;
+  const int j0 = imin(p.batch, lane * r.per), j1 = imin(p.batch, j0 + r.per);
+  r.mine = 0;
+  for (int j = j0; j < j1; ++j) r.mine += fp4_cost(fp4_len(p, p.seq_lens[j]));
+  int inc = r.mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(inc, d, 64);
+    if (lane >= d) inc += up;
+  }
+  r.before = inc - r.mine;
+  r.total = __builtin_amdgcn_readlane(inc, 63);
+  return r;
+}
 
-// NT column tiles of 16 rows; HALF: one tile, at most 8 rows, columns 8..15 carry the second terms
+// Workgroups resident per CU.  Two per CU with a tile read ahead per wave have 70 KB in flight, all that the memory
+// system takes; a third only makes more pieces to change over between (64 x 8192 tokens, head size 128: 96.5 us with two,
+// 104 with three).  Head size 64 has half the bytes per tile: 65.7 us with three, 69 with two, 75 with four.
+constexpr int fp4_wgs_per_cu(int head_dim, int rows) { return head_dim == 128 || rows > 16 ? 2 : 3; }
+
+// NT column tiles of 16 rows; HALF: one tile, at most 8 rows, columns 8..15 carry the probabilities' second terms
 template <int D, bool BF16, int NT, bool HALF>
 __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_kernel(const Fp4DecodeParams p) {
   static_assert(!HALF || NT == 1, "the half form has one tile");
-  constexpr int KS = D / 32;        // k-steps of the first product
-  constexpr int DT = D / 16;        // row tiles of the second
-  constexpr int VL = D / 64;        // 16-byte V loads per lane and tile
-  constexpr bool Q2 = !BF16 && !HALF;  // a second query term in registers of its own
+  constexpr int DT = D / 16;        // row tiles of the second product
+  constexpr int VW = D / 32;        // words of V codes per lane and page-half
+  constexpr int TERMS = BF16 ? 2 : 3;
+  // D = 64 fills half of the product's 128 columns: two terms share one product (K twice, the terms side by side)
+  constexpr int PRODUCTS = D == 128 ? TERMS : (TERMS + 1) / 2;
   constexpr int ROWS = HALF ? 8 : 16 * NT;
-  constexpr int COPIES = NT == 1 ? 4 : 1;  // LDS images of the waves' sums (more than 16 rows: one, added to in turn)
-  __shared__ float sm_o[COPIES][ROWS][D + 2];  // (+ 2: the 16 rows a wave writes at once start in different banks)
-  __shared__ float sm_ml[4][ROWS][2];
-  __shared__ int plan_sm[4 + 2];
+  __shared__ __attribute__((aligned(16))) float sm_o[4][ROWS][D + 4];  // (+ 4: the rows a wave writes at once start in different banks)
+  __shared__ f4_f32x2 sm_ml[4][ROWS];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
-  const int w = (int)blockIdx.x / p.Hkv;
-  const int h = (int)blockIdx.x - w * p.Hkv;
-  const DcPiece dp = dc_find_piece<256>(p.seq_lens, p.batch, p.Hkv, p.plan_slots, w, plan_sm, tid);
-  if (dp.b < 0) return;  // fewer pieces in this step than the grid provides for
-  const int b = __builtin_amdgcn_readfirstlane(dp.b);
-  const int n = __builtin_amdgcn_readfirstlane(dp.n);
-  const int tile0 = __builtin_amdgcn_readfirstlane(dp.tile0);
-  const int tile_end = tile0 + __builtin_amdgcn_readfirstlane(dp.ntiles);
-  const int R = p.m * p.G;
+  // Workgroups go round the 8 XCDs: this order gives an XCD a run of spans with all their heads, so that the heads of a
+  // page -- and the cache lines in which two heads' scale bytes meet -- are read through one L2 at about the same time
+  // (64 x 8192 tokens, 32 / 8 heads: 106.2 us against 108.6 with the heads spread over the XCDs).
+  const int lin = ((int)blockIdx.x & 7) * ((int)gridDim.x >> 3) + ((int)blockIdx.x >> 3);
+  const int w = lin / p.units, unit = lin - w * p.units;
+  const int h = unit / p.row_groups, row0 = 32 * (unit - h * p.row_groups);
+  if (w >= p.spans) return;
 
-  // ---- query rows: operand Q^T, lane column c16 = row, k-step i covers columns g D/4 + 8 i .. + 7.  Row r is position
-  // n - m + r / G, head h G + r % G. ----
-  uint4 qf[NT][KS], ql[Q2 ? NT : 1][KS];
-  int pos[NT];  // the position of this lane's row
+  // the request at which this workgroup's span begins, and where in it
+  int b, off, left;
+  {
+    const Fp4Plan plan = fp4_plan(p, lane);
+    const int span = fp4_span(plan.total, p.spans);
+    const long long begin_ = (long long)w * span;
+    if (begin_ >= plan.total) return;  // fewer spans in this step than the grid provides for
+    const int begin = (int)begin_;
+    const unsigned long long own = __ballot(begin >= plan.before && begin < plan.before + plan.mine);
+    const int src = __builtin_ctzll(own);  // (one lane holds it: begin < total)
+    b = src * plan.per;
+    int at = __builtin_amdgcn_readlane(plan.before, src);
+    for (;;) {
+      const int cj = fp4_cost(fp4_len(p, fp4_sload(p.seq_lens + b)));
+      if (begin < at + cj) break;
+      at += cj;
+      ++b;
+    }
+    off = begin - at - kFp4Begin;  // (negative: the request begins in this span)
+    left = imin(plan.total - begin, span);
+  }
+  const int R = imin(p.m * p.G - row0, ROWS);  // this workgroup's rows: row0 .. row0 + R - 1 of the head
+  const int ps = 1 << p.page_shift;
+  const int64_t head_codes = (int64_t)h * ps * (D / 2);
+  const int scales_from_codes = (int)(fp4_code_bytes(p.Hkv, ps, D) + (int64_t)h * ps * (D / 32) - head_codes);
+  // byte offsets of a lane inside a page-half of a head
+  const int k_lane = c16 * (D / 2) + (D == 128 ? g : g & 1) * 16;
+  const int v_lane = D == 128 ? g * 256 + c16 * 16 : (g >> 1) * 256 + c16 * 16 + (g & 1) * 8;
+  const int ks_lane = (D == 128 ? g : g & 1) * ps + c16;
+  const int vs_lane = (D == 128 ? c16 >> 2 : c16 >> 3) * ps + 4 * g;
+
+  struct Raw {
+    fp4_u32x4 k[2];                  // 32 codes of key 16 t + c16
+    unsigned v[2 * VW];              // codes of keys 4 g .. + 3 and 16 + 4 g .. + 3, D / 16 columns each
+    unsigned ks[2];                  // scale bytes
+    unsigned vs[2];                  // four keys' scale bytes each
+    unsigned bad;                    // bit x: half x has no page
+  };
+  struct Pages {
+    int e0, e1;
+  };
+  // The piece of a request that is being computed: keys, tiles tile0 .. tile_end - 1, of which every row attends to all keys
+  // of those before full_end
+  int n, tile_end, full_end, t0;
+  bool whole;
+  const int32_t* bt;
+  uint4 qraw[NT][D / 32];  // (asked for one piece ahead as long as the registers allow)
+  constexpr bool QAHEAD = NT == 1;
+  Raw ring[2];  // the tile that is computed and the next one
+  Pages pg{0, 0};
+
+  // The pages of a tile, looked up a tile ahead of its loads.
+  auto pages_of = [&](int tile, Pages& pg) {
+    const int key0 = tile * kBlockN;
+    const int key1 = key0 + 16 < n ? key0 + 16 : key0;  // a half past the end reads the first one again
+    const int blk0 = key0 >> p.page_shift, blk1 = key1 >> p.page_shift;
+    pg.e0 = blk0 < p.max_blocks ? fp4_sload(bt + blk0) : -1;
+    pg.e1 = blk1 < p.max_blocks ? fp4_sload(bt + blk1) : -1;
+  };
+  auto load = [&](int tile, const Pages& pg, Raw& r) {
+    const int key0 = tile * kBlockN;
+    const int key1 = key0 + 16 < n ? key0 + 16 : key0;
+    r.bad = ((unsigned)pg.e0 >= (unsigned)p.num_pages ? 1u : 0u) | ((unsigned)pg.e1 >= (unsigned)p.num_pages ? 2u : 0u);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int r = HALF ? (c16 & 7) : 16 * t + c16;
-    const bool row = r < R;
-    const int j = row ? r / p.G : 0, hd = h * p.G + (row ? r - j * p.G : 0);
-    pos[t] = n - p.m + j;
-    const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + ((int64_t)b * p.m + j) * p.q_stride_t + hd * p.q_stride_h;
+    for (int x = 0; x < 2; ++x) {
+      const int e = (r.bad >> x) & 1 ? 0 : (x ? pg.e1 : pg.e0);
+      const int at = (x ? key1 : key0) & (ps - 1);
+      const int64_t base = e * p.stride_page + head_codes + at * (D / 2);
+      const int scales = scales_from_codes + at - at * (D / 2);
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.k) + base, 0, 0x7fffffff, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.v) + base, 0, 0x7fffffff, 0x00020000);
+      constexpr int kStream = 2;  // codes are read once: non-temporal (96 against 112 us for the loads of 64 x 8192)
+      r.k[x] = __builtin_bit_cast(fp4_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_lane, 0, kStream));
+      if constexpr (D == 128) {
+        const fp4_u32x4 y = __builtin_bit_cast(fp4_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, v_lane, 0, kStream));
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      uint4 x = *reinterpret_cast<const uint4*>(src + g * (D / 4) + 8 * i);
-      if (!row) x = make_uint4(0, 0, 0, 0);
-      if constexpr (BF16) {
-        qf[t][i] = x;
+        for (int i = 0; i < 4; ++i) r.v[4 * x + i] = y[i];
       } else {
-        const unsigned xs[4] = {x.x, x.y, x.z, x.w};
+        const fp4_u32x2 y = __builtin_bit_cast(fp4_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, v_lane, 0, kStream));
+        r.v[2 * x] = y[0];
+        r.v[2 * x + 1] = y[1];
+      }
+      r.ks[x] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(rk, ks_lane, scales, 0);
+      r.vs[x] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rv, vs_lane, scales, 0);
+    }
+  };
+  // Lane column c16 = query row; the 8-bit operand of the product holds columns 16 g .. + 15 and 64 + 16 g .. + 15 of it.
+  // Row r is position n - m + r / G, head h G + r % G.
+  auto load_q = [&]() {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int x = HALF ? (c16 & 7) : 16 * t + c16;
+      const int r = row0 + (x < R ? x : 0);  // (columns without a row repeat the first)
+      const int j = r / p.G, hd = h * p.G + (r - j * p.G);
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + ((int64_t)b * p.m + j) * p.q_stride_t + hd * p.q_stride_h;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) qraw[t][i] = *reinterpret_cast<const uint4*>(src + 64 * (i >> 1) + 16 * g + 8 * (i & 1));
+    }
+  };
+  // The next piece of the span: its query rows and first tiles are asked for here, before the one that ends is written out.
+  auto start = [&]() {
+    n = fp4_len(p, fp4_sload(p.seq_lens + b));
+    const int tiles = fp4_tiles(n), take = imin(left, tiles - off);
+    left -= take;
+    tile_end = off + take;
+    off = imax(off, 0);
+    whole = off == 0 && tile_end == tiles;
+    full_end = imin(tile_end, imax(0, n - p.m + 1) / kBlockN);
+    t0 = off + wave;
+    bt = p.block_table + b * p.block_table_stride;
+    if constexpr (QAHEAD) load_q();
+    if (t0 < tile_end) {
+      pages_of(t0, pg);
+      load(t0, pg, ring[0]);
+    }
+    if (t0 + 4 < tile_end) pages_of(t0 + 4, pg);
+  };
+
+  if (left + imin(off, 0) <= 0) return;  // (the span holds no more than a request's beginning)
+  start();
+  for (;;) {
+    if constexpr (!QAHEAD) load_q();
+    // ---- the query's terms: x = 2^E (t0 + t1 / 16 + t2 / 256), E such that the block's largest lies in [128, 256) 2^E ----
+    f4_i32x8 qt[NT][PRODUCTS];
+    int qs[NT][PRODUCTS];  // scale bytes: lane (c16, g) gives the one of columns 32 g .. of the product
+    int pos[NT];           // the position of this lane's row
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int row = HALF ? (c16 & 7) : 16 * t + c16;
+      pos[t] = n - p.m + (row0 + (row < R ? row : 0)) / p.G;
+      unsigned w[D / 8];  // two columns each
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) w[4 * i] = qraw[t][i].x, w[4 * i + 1] = qraw[t][i].y, w[4 * i + 2] = qraw[t][i].z, w[4 * i + 3] = qraw[t][i].w;
+      int E[D / 64];
+      bool bad = false;
+#pragma unroll
+      for (int y = 0; y < D / 64; ++y) {
+        f4_u16x2 top = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(f4_u16x2, w[8 * y + i] & 0x7fff7fffu));
+        unsigned m = max((unsigned)top[0], (unsigned)top[1]);
+        m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));  // the block's other 16 columns
+        bad |= m >= (BF16 ? 0x7f80u : 0x7c00u);
+        const unsigned bits = BF16 ? m << 16 : __float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)m));
+        E[y] = imin(imax((int)(bits >> 23) - 127 - 7, -118), 120);
+      }
+      // lane group g's block of the product: its exponent is with the lanes that hold the block's columns
+      {
+        const int src = c16 + 32 * (g & 1);
+        const int lo = __shfl(E[0], src, 64);
+        if constexpr (D == 128) {
+          const int hi = __shfl(E[D / 64 - 1], src, 64);
+          const int mine = g < 2 ? lo : hi;
+#pragma unroll
+          for (int z = 0; z < PRODUCTS; ++z) qs[t][z] = mine + 127 - 4 * z;
+        } else {
+#pragma unroll
+          for (int z = 0; z < PRODUCTS; ++z) qs[t][z] = lo + 127 - 4 * (2 * z + (g >> 1));
+        }
+      }
+#pragma unroll
+      for (int z = 0; z < PRODUCTS; ++z) qt[t][z] = f4_i32x8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {  // four columns
+        float rest[4];
+#pragma unroll
+        for (int z = 0; z < TERMS; ++z) {
+          const float scale = __uint_as_float((unsigned)(E[i / 4] + 127 - 4 * z) << 23);
+          f4_s16x2 word = {0, 0};
+          if (z == 0) {
+            if constexpr (BF16) {
+              word = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(word, __builtin_bit_cast(fp4_bf16x2, w[2 * i]), scale, false);
+              word = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(word, __builtin_bit_cast(fp4_bf16x2, w[2 * i + 1]), scale, true);
+            } else {
+              word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(word, __builtin_bit_cast(fp4_f16x2, w[2 * i]), scale, false);
+              word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(word, __builtin_bit_cast(fp4_f16x2, w[2 * i + 1]), scale, true);
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              if constexpr (BF16) {
+                rest[2 * y] = __uint_as_float(w[2 * i + y] << 16);
+                rest[2 * y + 1] = __uint_as_float(w[2 * i + y] & 0xffff0000u);
+              } else {
+                const fp4_f16x2 f = __builtin_bit_cast(fp4_f16x2, w[2 * i + y]);
+                rest[2 * y] = (float)f[0];
+                rest[2 * y + 1] = (float)f[1];
+              }
+            }
+          } else {
+            word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(word, rest[0], rest[1], scale, false);
+            word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(word, rest[2], rest[3], scale, true);
+          }
+          const unsigned bits = __builtin_bit_cast(unsigned, word);
+          if (z + 1 < TERMS) {
+            const f4_f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(bits, scale, false), c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(bits, scale, true);
+            rest[0] -= a[0];
+            rest[1] -= a[1];
+            rest[2] -= c[0];
+            rest[3] -= c[1];
+          }
+          if constexpr (D == 128) qt[t][z][i] = (int)bits;
+          else qt[t][z / 2][4 * (z & 1) + i] = (int)bits;
+        }
+      }
+      if (__any(bad)) {  // an infinity or a NaN: the row's scores are NaN
+        asm volatile("");
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qt[t][0][i] = bad ? 0x7f7f7f7f : qt[t][0][i];
+      }
+    }
+
+    f4_f32x4 o[NT][DT], l[NT];
+    float mx[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      mx[t] = kFp4MinusBig;
+      l[t] = f4_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < DT; ++i) o[t][i] = f4_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // The conversion takes the exponent field of its scale alone: the byte moved there, whatever lies around it.
+    auto scale_of = [](unsigned word, int byte) -> float { return __uint_as_float(byte < 3 ? word << (23 - 8 * byte) : word >> 1); };
+
+    // ---- O^T += V^T P^T with the probabilities in pb (and their second terms in pl unless HALF), one byte of every
+    // key's codes -- a pair of columns, two row tiles -- at a time; and the probabilities' sums ----
+    auto weighted_sum = [&](const Raw& r, const uint4 (&pb)[NT], const uint4 (&pl)[NT]) {
+      const f4_bf16x8 ones = __builtin_bit_cast(f4_bf16x8, make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        l[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(f4_bf16x8, pb[t]), l[t], 0, 0, 0);
+        if constexpr (!HALF) l[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(f4_bf16x8, pl[t]), l[t], 0, 0, 0);
+      }
+      float sc[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sc[j] = scale_of(r.vs[j >> 2], j & 3);
+      auto pair = [&](auto at) {
+        constexpr int B = decltype(at)::value;
+        unsigned c[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if constexpr (D == 128) c[j] = fp4_bf16<B>(r.v[j], sc[j]);
+          else c[j] = (j & 1) ? fp4_bf16<2 + (B & 1)>(r.v[j >> 1], sc[j]) : fp4_bf16<B & 1>(r.v[j >> 1], sc[j]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const unsigned sel = e ? 0x07060302u : 0x05040100u;
+          const f4_bf16x8 av = __builtin_bit_cast(f4_bf16x8, make_uint4(
+              __builtin_amdgcn_perm(c[1], c[0], sel), __builtin_amdgcn_perm(c[3], c[2], sel),
+              __builtin_amdgcn_perm(c[5], c[4], sel), __builtin_amdgcn_perm(c[7], c[6], sel)));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            f4_f32x4& d = o[t][2 * B + e];
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(f4_bf16x8, pb[t]), d, 0, 0, 0);
+            if constexpr (!HALF) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(f4_bf16x8, pl[t]), d, 0, 0, 0);
+          }
+        }
+      };
+      pair(std::integral_constant<int, 0>{});
+      pair(std::integral_constant<int, 1>{});
+      if constexpr (D == 128) {
+        pair(std::integral_constant<int, 2>{});
+        pair(std::integral_constant<int, 3>{});
+      }
+    };
+    // takes key j (of the lane's 8) out of V
+    auto drop_key = [&](Raw& r, int j) {
+      if constexpr (D == 128) r.v[j] = 0;
+      else r.v[j >> 1] &= (j & 1) ? 0x0000ffffu : 0xffff0000u;
+      r.vs[j >> 2] &= ~(0xffu << (8 * (j & 3)));
+    };
+
+    // TAIL: the tile may hold keys past a row's position, or past the sequence (their V must not enter even as 0 x NaN)
+    auto process = [&](auto tail_, Raw& r, int tile) {
+      constexpr bool TAIL = decltype(tail_)::value;
+      const int key0 = tile * kBlockN + 4 * g;  // the lane's keys: key0 + 16 (j / 4) + j % 4
+      if (r.bad) {  // keys without a page count as NaN
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if ((r.bad >> x) & 1) r.ks[x] = 0xffu, r.vs[x] = ~0u;
+      }
+      // scores
+      f4_f32x4 s[NT][2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const f4_i32x8 a = {(int)r.k[x][0], (int)r.k[x][1], (int)r.k[x][2], (int)r.k[x][3], 0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          s[t][x] = f4_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int z = PRODUCTS - 1; z >= 0; --z)  // (small terms first)
+            s[t][x] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qt[t][z], s[t][x], 4, 0, 0, (int)r.ks[x], 0, qs[t][z]);
+        }
+      }
+      // The product does not turn a scale byte of 255 into NaN: such keys' scores are set.  (Lane (c16, .) holds scale
+      // bytes of key c16, lane (., g) the scores of keys 4 g ..)
+      if (__any(imax((int)r.ks[0], (int)r.ks[1]) == 255)) {
+        asm volatile("");  // (kept behind its branch: the compiler would rather compute it for every tile)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          unsigned long long nan = __ballot(r.ks[x] == 255u);
+          nan |= nan >> 32;
+          nan |= nan >> 16;
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if ((nan >> (4 * g + y)) & 1)
+#pragma unroll
+              for (int t = 0; t < NT; ++t) s[t][x][y] = __builtin_nanf("");
+        }
+      }
+      if (TAIL && tile * kBlockN + kBlockN > n) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (key0 + 16 * (j >> 2) + (j & 3) >= n) drop_key(r, j);
+      }
+      if (TAIL && p.m > 1) {
+        // A NaN in V at a position that only some rows may see must not reach the others as 0 x NaN: such blocks are
+        // taken out, and the rows that see them set to NaN.  (Lane (c16, g) holds V of column block c16 / (512 / D) and
+        // outputs of block g D / 128.)
+        unsigned nan = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) nan |= ((r.vs[j >> 2] >> (8 * (j & 3))) & 0xffu) == 0xffu ? 1u << j : 0u;
+        if (__any(nan != 0)) {
+          const unsigned long long mine = D == 128 ? 0x000f000f000f000full << (4 * g) : 0x00ff00ff00ff00ffull << (8 * (g >> 1));
+          for (int at = 0; at < p.m; ++at) {
+            const int last = n - p.m + at;
+            unsigned upto = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) upto |= key0 + 16 * (j >> 2) + (j & 3) <= last ? 1u << j : 0u;
+            const bool hit = (__ballot((nan & upto) != 0) & mine) != 0;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              if (hit && pos[t] == last)
+#pragma unroll
+                for (int i = 0; i < DT; ++i) o[t][i] = f4_f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if ((nan >> j) & 1) drop_key(r, j);
+        }
+      }
+      uint4 pb[NT], pl[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = s[t][j >> 2][j & 3];
+        if constexpr (TAIL) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (key0 + 16 * (j >> 2) + (j & 3) > pos[t]) x[j] = -__builtin_inff();
+        }
+        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * p.scale_log2;
+        if (__any(top > mx[t] + kFp4Slack)) {
+          float m2 = fmaxf(top, __shfl_xor(top, 16, 64));
+          m2 = fmaxf(m2, __shfl_xor(m2, 32, 64));
+          m2 = fmaxf(m2, mx[t]);
+          const float f = fp4_exp2(mx[t] - m2);
+          mx[t] = m2;
+          l[t] *= f;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) o[t][i] *= f;
+        }
+        float pr[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pr[j] = fp4_exp2(__builtin_fmaf(x[j], p.scale_log2, -mx[t]));
         unsigned hi[4], lo[4];
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          const fp4_f16x2 f = __builtin_bit_cast(fp4_f16x2, xs[y]);
-          hi[y] = fp4_pack_bf16((float)f[0], (float)f[1]);
-          // (an infinity has no second term)
-          const float h0 = __uint_as_float(hi[y] << 16), h1 = __uint_as_float(hi[y] & 0xffff0000u);
-          const float d0 = (float)f[0] - h0, d1 = (float)f[1] - h1;
-          lo[y] = fp4_pack_bf16(__builtin_isinf(h0) ? 0.f : d0, __builtin_isinf(h1) ? 0.f : d1);
+          hi[y] = fp4_pack_bf16(pr[2 * y], pr[2 * y + 1]);
+          const float d0 = pr[2 * y] - __uint_as_float(hi[y] << 16), d1 = pr[2 * y + 1] - __uint_as_float(hi[y] & 0xffff0000u);
+          lo[y] = fp4_pack_bf16(d0, d1);
+          if constexpr (HALF) hi[y] = c16 < 8 ? hi[y] : lo[y];
         }
-        const uint4 a = make_uint4(hi[0], hi[1], hi[2], hi[3]), c = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if constexpr (HALF) qf[t][i] = c16 < 8 ? a : c;
-        else qf[t][i] = a, ql[Q2 ? t : 0][i] = c;
+        pb[t] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        pl[t] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
-    }
-  }
-
-  // ---- addresses.  A tile's two 16-key halves may lie on two pages; K rows of a lane belong to half m / 8, its V keys to
-  // half g / 2. ----
-  const int ps = 1 << p.page_shift;
-  const int64_t codes = fp4_code_bytes(p.Hkv, ps, D);
-  const int64_t head_codes = (int64_t)h * ps * (D / 2);
-  const int64_t head_scales = codes + (int64_t)h * ps * (D / 32);
-  const int32_t* const bt = p.block_table + b * p.block_table_stride;
-  const bool khalf = (c16 & 8) != 0, vhalf = (g & 2) != 0;
-  const int k_lane = (8 * ((c16 >> 2) & 1) + (c16 & 3)) * (D / 2) + g * (D / 8);
-  const int v_lane = (g & 1) * (8 * (D / 2)) + c16 * 16;
-  const int ks_lane = (D == 128 ? g : g >> 1) * ps + 8 * ((c16 >> 2) & 1);
-  const int vs_lane = (D == 128 ? c16 >> 2 : c16 >> 3) * ps + 8 * (g & 1);
-
-  struct Raw {
-    fp4_u32x4 k[2];  // D = 64: the first two words
-    fp4_u32x4 v[VL];
-    fp4_u32x2 ks, vs;
-    unsigned bad;  // bit x: half x has no page
-  };
-  auto load = [&](int tile, Raw& r) {
-    const int key0 = tile * kBlockN;
-    const int blk0 = key0 >> p.page_shift;
-    const int key1 = key0 + 16 < n ? key0 + 16 : key0;  // a half past the end reads the first one again
-    const int blk1 = key1 >> p.page_shift;
-    int e0 = blk0 < p.max_blocks ? fp4_sload(bt + blk0) : -1;
-    int e1 = blk1 < p.max_blocks ? fp4_sload(bt + blk1) : -1;
-    r.bad = ((unsigned)e0 >= (unsigned)p.num_pages ? 1u : 0u) | ((unsigned)e1 >= (unsigned)p.num_pages ? 2u : 0u);
-    if (r.bad & 1) e0 = 0;
-    if (r.bad & 2) e1 = 0;
-    const int at0 = key0 & (ps - 1), at1 = key1 & (ps - 1);
-    const int64_t o0 = e0 * p.stride_page, o1 = e1 * p.stride_page;
-    const int64_t c0 = o0 + head_codes + at0 * (D / 2), c1 = o1 + head_codes + at1 * (D / 2);
-    const int64_t s0 = o0 + head_scales + at0, s1 = o1 + head_scales + at1;
-    const uint8_t* kp = p.k + (khalf ? c1 : c0) + k_lane;
-    const uint8_t* vp = p.v + (vhalf ? c1 : c0) + v_lane;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if constexpr (D == 128) {
-        r.k[t] = __builtin_nontemporal_load(reinterpret_cast<const fp4_u32x4*>(kp + t * 4 * (D / 2)));
-      } else {
-        const fp4_u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const fp4_u32x2*>(kp + t * 4 * (D / 2)));
-        r.k[t] = fp4_u32x4{x[0], x[1], 0, 0};
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < VL; ++x) r.v[x] = __builtin_nontemporal_load(reinterpret_cast<const fp4_u32x4*>(vp + x * 256));
-    r.ks = *reinterpret_cast<const fp4_u32x2*>(p.k + (khalf ? s1 : s0) + ks_lane);
-    r.vs = *reinterpret_cast<const fp4_u32x2*>(p.v + (vhalf ? s1 : s0) + vs_lane);
-  };
-
-  f4_f32x4 o[NT][DT];
-  float mx[NT], l[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    mx[t] = kFp4MinusBig;
-    l[t] = 0.f;
-#pragma unroll
-    for (int i = 0; i < DT; ++i) o[t][i] = f4_f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  auto scale_of = [](unsigned word, int byte) -> float { return __uint_as_float(((word >> (8 * byte)) & 0xffu) << 23); };
-
-  // ---- O^T += V^T P^T with the probabilities in pb (and their second terms in pl unless HALF), one byte of every
-  // key's codes -- a pair of columns, two row tiles -- at a time ----
-  auto weighted_sum = [&](const Raw& r, const uint4 (&pb)[NT], const uint4 (&pl)[NT]) {
-    float sc[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sc[j] = scale_of(r.vs[j >> 2], j & 3);
-    auto pair = [&](auto at) {
-      constexpr int B = decltype(at)::value;
-      unsigned c[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if constexpr (D == 128) c[j] = fp4_bf16<B>(r.v[j >> 2][j & 3], sc[j]);
-        else c[j] = (j & 1) ? fp4_bf16<2 + (B & 1)>(r.v[0][j >> 1], sc[j]) : fp4_bf16<B & 1>(r.v[0][j >> 1], sc[j]);
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const unsigned sel = e ? 0x07060302u : 0x05040100u;
-        const f4_bf16x8 av = __builtin_bit_cast(f4_bf16x8, make_uint4(
-            __builtin_amdgcn_perm(c[1], c[0], sel), __builtin_amdgcn_perm(c[3], c[2], sel),
-            __builtin_amdgcn_perm(c[5], c[4], sel), __builtin_amdgcn_perm(c[7], c[6], sel)));
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          f4_f32x4& d = o[t][2 * B + e];
-          d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(f4_bf16x8, pb[t]), d, 0, 0, 0);
-          if constexpr (!HALF) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(f4_bf16x8, pl[t]), d, 0, 0, 0);
-        }
-      }
+      weighted_sum(r, pb, pl);
     };
-    pair(std::integral_constant<int, 0>{});
-    pair(std::integral_constant<int, 1>{});
-    if constexpr (D == 128) {
-      pair(std::integral_constant<int, 2>{});
-      pair(std::integral_constant<int, 3>{});
-    }
-  };
-  // takes key j (of the lane's 8) out of V
-  auto drop_key = [&](Raw& r, int j) {
-    if constexpr (D == 128) r.v[j >> 2][j & 3] = 0;
-    else r.v[0][j >> 1] &= (j & 1) ? 0x0000ffffu : 0xffff0000u;
-    r.vs[j >> 2] &= ~(0xffu << (8 * (j & 3)));
-  };
 
-  auto process = [&](Raw& r, int tile) {
-    const int key0 = tile * kBlockN;
-    if (r.bad) {  // keys without a page count as NaN
-      if ((r.bad >> (khalf ? 1 : 0)) & 1) r.ks = fp4_u32x2{~0u, ~0u};
-      if ((r.bad >> (vhalf ? 1 : 0)) & 1) r.vs = fp4_u32x2{~0u, ~0u};
-    }
-    // scores
-    f4_f32x4 s[NT][2];
+    if (t0 < full_end) {
+      for (;;) {
+        bool done = false;
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-      const float sc = __uint_as_float(((r.ks[tt] >> (8 * (c16 & 3))) & 0xffu) << 23);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) s[t][tt] = f4_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        const unsigned word = r.k[tt][i];
-        const uint4 a = make_uint4(fp4_bf16<0>(word, sc), fp4_bf16<1>(word, sc), fp4_bf16<2>(word, sc), fp4_bf16<3>(word, sc));
-        const f4_bf16x8 av = __builtin_bit_cast(f4_bf16x8, a);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          s[t][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(f4_bf16x8, qf[t][i]), s[t][tt], 0, 0, 0);
-          if constexpr (Q2) s[t][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(f4_bf16x8, ql[t][i]), s[t][tt], 0, 0, 0);
+        for (int x = 0; x < 2; ++x) {
+          if (t0 + 4 < tile_end) load(t0 + 4, pg, ring[1 - x]);
+          if (t0 + 8 < tile_end) pages_of(t0 + 8, pg);
+          process(std::false_type{}, ring[x], t0);
+          t0 += 4;
+          if (t0 >= full_end) {
+            if (x == 0) ring[0] = ring[1];
+            done = true;
+            break;
+          }
         }
+        if (done) break;
       }
     }
-    // the tile may hold keys past a row's position (or past the sequence: their V must not enter even as 0 x NaN)
-    const bool tail = key0 + kBlockN > n - p.m + 1;
-    if (key0 + kBlockN > n) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (key0 + 8 * g + j >= n) drop_key(r, j);
-    }
-    if (p.m > 1 && tail) {
-      // A NaN in V at a position that only some rows may see must not reach the others as 0 x NaN: such blocks are taken
-      // out, and the rows that see them set to NaN.  (Lane (c16, g) holds V of column block c16 / (512 / D) and outputs of
-      // block g D / 128.)
-      unsigned nan = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) nan |= ((r.vs[j >> 2] >> (8 * (j & 3))) & 0xffu) == 0xffu ? 1u << j : 0u;
-      if (__any(nan != 0)) {
-        const unsigned long long mine = D == 128 ? 0x000f000f000f000full << (4 * g) : 0x00ff00ff00ff00ffull << (8 * (g >> 1));
-        for (int at = 0; at < p.m; ++at) {
-          const int last = n - p.m + at, seen = last - key0 - 8 * g;  // the lane's keys 0 .. seen
-          const unsigned upto = seen < 0 ? 0u : (seen >= 7 ? 0xffu : (2u << seen) - 1u);
-          const bool hit = (__ballot((nan & upto) != 0) & mine) != 0;
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-            if (hit && pos[t] == last)
-#pragma unroll
-              for (int i = 0; i < DT; ++i) o[t][i] = f4_f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if ((nan >> j) & 1) drop_key(r, j);
+    while (t0 < tile_end) {  // (the first of them is loaded already; more than one only where rows end in several tiles)
+      process(std::true_type{}, ring[0], t0);
+      t0 += 4;
+      if (t0 < tile_end) {
+        pages_of(t0, pg);
+        load(t0, pg, ring[0]);
       }
     }
-    uint4 pb[NT], pl[NT];
+
+    // ---- the piece is done; the next one's loads go out before it is written ----
+    const int b_done = b, n_done = n;
+    const bool whole_done = whole, more = left > kFp4Begin;
+    if (more) {
+      off = -kFp4Begin;
+      do ++b;
+      while (fp4_sload(p.seq_lens + b) <= 0);  // (tiles are left, so a request follows)
+      start();
+    }
+
+    // ---- join the waves ----
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      float x[8];
+      float sum = l[t][0];
+      if constexpr (HALF) {
+        sum += fp4_other8(sum);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float v = s[t][j >> 2][j & 3];
-        if constexpr (HALF && !BF16) v += fp4_other8(v);  // the query's two terms
-        x[j] = v;
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) o[t][i][y] += fp4_other8(o[t][i][y]);
       }
-      if (tail) {
+      const int r = HALF ? c16 : 16 * t + c16;
+      if (r < ROWS) {
+        if (g == 0) sm_ml[wave][r] = f4_f32x2{mx[t], sum};
+        // O^T tile i: row 4 g + y of it is column (4 g + y) D/16 + i
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (key0 + 8 * g + j > pos[t]) x[j] = -__builtin_inff();
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int i = 0; i < DT; i += 4)
+            *reinterpret_cast<f4_f32x4*>(&sm_o[wave][r][(4 * g + y) * DT + i]) = f4_f32x4{o[t][i][y], o[t][i + 1][y], o[t][i + 2][y], o[t][i + 3][y]};
       }
-      const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * p.scale_log2;
-      if (__any(top > mx[t] + kFp4Slack)) {
-        float m2 = fmaxf(top, __shfl_xor(top, 16, 64));
-        m2 = fmaxf(m2, __shfl_xor(m2, 32, 64));
-        m2 = fmaxf(m2, mx[t]);
-        const float f = fp4_exp2(mx[t] - m2);
-        mx[t] = m2;
-        l[t] *= f;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) o[t][i] *= f;
-      }
-      float pr[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pr[j] = fp4_exp2(__builtin_fmaf(x[j], p.scale_log2, -mx[t]));
-      l[t] += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
-      unsigned hi[4], lo[4];
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        hi[y] = fp4_pack_bf16(pr[2 * y], pr[2 * y + 1]);
-        const float d0 = pr[2 * y] - __uint_as_float(hi[y] << 16), d1 = pr[2 * y + 1] - __uint_as_float(hi[y] & 0xffff0000u);
-        lo[y] = fp4_pack_bf16(d0, d1);
-        if constexpr (HALF) hi[y] = c16 < 8 ? hi[y] : lo[y];
-      }
-      pb[t] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      pl[t] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-    weighted_sum(r, pb, pl);
-  };
-
-  // ---- the wave's tiles, the next one's loads in flight while one is computed ----
-  {
-    int t = tile0 + wave;
-    Raw a, c;
-    if (t < tile_end) {
-      load(t, a);
-      for (;;) {
-        if (t + 4 < tile_end) load(t + 4, c);
-        process(a, t);
-        t += 4;
-        if (t >= tile_end) break;
-        if (t + 4 < tile_end) load(t + 4, a);
-        process(c, t);
-        t += 4;
-        if (t >= tile_end) break;
-      }
-    }
-  }
-
-  // ---- join the waves ----
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    l[t] += __shfl_xor(l[t], 16, 64);
-    l[t] += __shfl_xor(l[t], 32, 64);
-    if constexpr (HALF) {
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) o[t][i][y] += fp4_other8(o[t][i][y]);
-    }
-    const int r = HALF ? c16 : 16 * t + c16;
-    if (g == 0 && r < ROWS) {
-      sm_ml[wave][r][0] = mx[t];
-      sm_ml[wave][r][1] = l[t];
-    }
-  }
-  __syncthreads();
-  // Row r's common maximum, and this wave's factor.  A wave without tiles holds (lowest, 0): factor 0 or, if no wave saw
-  // a key, 1 on zeros.
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int r = HALF ? (c16 & 7) : 16 * t + c16;
-    const float top = fmaxf(fmaxf(sm_ml[0][r][0], sm_ml[1][r][0]), fmaxf(sm_ml[2][r][0], sm_ml[3][r][0]));
-    const float f = fp4_exp2(mx[t] - top);
-#pragma unroll
-    for (int i = 0; i < DT; ++i) o[t][i] *= f;
-  }
-  // O^T tile i: row 4 g + y of it is column (4 g + y) D/16 + i
-  if constexpr (COPIES == 4) {
-    const int r = c16;
-    if (r < ROWS) {
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) sm_o[wave][r][(4 * g + y) * DT + i] = o[0][i][y];
     }
     __syncthreads();
-  } else {
-    for (int turn = 0; turn < 4; ++turn) {
-      if (wave == turn) {
+    for (int u = tid; u < R * (D / 4); u += 256) {
+      const int r = u / (D / 4), d = 4 * (u % (D / 4));
+      const int j = (row0 + r) / p.G, hd = h * p.G + (row0 + r - j * p.G);
+      // The row's common maximum and every wave's factor.  A wave without tiles holds (lowest, 0): factor 0 or, if no wave
+      // saw a key, 1 on zeros.
+      f4_f32x2 ml[4];
+      float top = kFp4MinusBig, ls = 0.f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              float* d = &sm_o[0][16 * t + c16][(4 * g + y) * DT + i];
-              *d = turn == 0 ? o[t][i][y] : *d + o[t][i][y];
-            }
+      for (int wv = 0; wv < 4; ++wv) {
+        ml[wv] = sm_ml[wv][r];
+        top = fmaxf(top, ml[wv][0]);
       }
-      __syncthreads();
-    }
-  }
-  for (int u = tid; u < R * D; u += 256) {
-    const int r = u / D, d = u - r * D;
-    const int j = r / p.G, hd = h * p.G + (r - j * p.G);
-    if (n - p.m + j < 0) continue;  // the sequence is shorter than the step's rows: no such position
-    float top = kFp4MinusBig, sum = 0.f, x = 0.f;
+      f4_f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int wv = 0; wv < 4; ++wv) top = fmaxf(top, sm_ml[wv][r][0]);
+      for (int wv = 0; wv < 4; ++wv) {
+        const float f = fp4_exp2(ml[wv][0] - top);
+        ls += ml[wv][1] * f;
+        x += *reinterpret_cast<const f4_f32x4*>(&sm_o[wv][r][d]) * f;
+      }
+      if (n_done - p.m + j < 0) continue;  // the sequence is shorter than the step's rows: no such position
+      if (whole_done) {
+        const float inv = 1.f / ls;
+        const int64_t at = ((int64_t)b_done * p.m + j) * p.out_stride_t + hd * p.out_stride_h + d;
 #pragma unroll
-    for (int wv = 0; wv < 4; ++wv) sum += sm_ml[wv][r][1] * fp4_exp2(sm_ml[wv][r][0] - top);
-#pragma unroll
-    for (int y = 0; y < COPIES; ++y) x += sm_o[y][r][d];
-    if (dp.pieces == 1) {
-      fp4_store_out(p.out, ((int64_t)b * p.m + j) * p.out_stride_t + hd * p.out_stride_h + d, x / sum, p.out_f32 != 0, BF16);
-    } else {
-      const int64_t slot = ((int64_t)w * p.m + j) * p.H + hd;
-      p.partial_o[slot * D + d] = x;
-      if (d == 0) {
-        p.partial_ml[2 * slot] = top;
-        p.partial_ml[2 * slot + 1] = sum;
+        for (int y = 0; y < 4; ++y) fp4_store_out(p.out, at + y, x[y] * inv, p.out_f32 != 0, BF16);
+      } else {
+        const int64_t slot = ((int64_t)(w + b_done) * p.m + j) * p.H + hd;
+        *reinterpret_cast<f4_f32x4*>(p.partial_o + slot * D + d) = x;
+        if (d == 0) *reinterpret_cast<f4_f32x2*>(p.partial_ml + 2 * slot) = f4_f32x2{top, ls};
       }
     }
+    if (!more) return;
+    __syncthreads();  // (the next piece's sums go to the same LDS)
   }
 }
 
-// Joins the pieces of one output row: one workgroup per (request, row, head), D / 4 lanes along the columns, 1024 / D
-// pieces at a time.
-template <int D, bool BF16>
-__global__ __launch_bounds__(256) void fp4_join_kernel(const Fp4DecodeParams p) {
-  constexpr int LANES = D / 4, AT_ONCE = 256 / LANES;
-  __shared__ int sm[4 + 2];
-  __shared__ float sm_m[AT_ONCE], sm_l[AT_ONCE];
-  __shared__ float sm_o[AT_ONCE][D];
-  const int tid = threadIdx.x;
-  const int b = blockIdx.y, j = (int)blockIdx.x / p.H, hd = (int)blockIdx.x - j * p.H;
-  const int n = p.seq_lens[b];
-  if (n <= 0 || n - p.m + j < 0) return;
-  // first piece of request b, and how many it has
-  int before = 0, all = 0;
-  for (int x = tid; x < p.batch; x += 256) all += dc_tiles_of(p.seq_lens[x]);
-  const int P = dc_piece_len(dc_block_sum<256>(all, sm, tid), p.Hkv, p.plan_slots);
-  const int pieces = (dc_tiles_of(n) + P - 1) / P;
+// Joins the pieces of output rows, D / 4 lanes along a row, PIECES of its pieces at a time.
+template <int D, bool BF16, int PIECES>
+__global__ __launch_bounds__(D / 4 * PIECES < 256 ? 256 : D / 4 * PIECES) void fp4_join_kernel(const Fp4DecodeParams p) {
+  constexpr int LANES = D / 4, THREADS = LANES * PIECES < 256 ? 256 : LANES * PIECES, ROWS = THREADS / (LANES * PIECES);
+  __shared__ float sm_ml[ROWS][PIECES][2];
+  __shared__ float sm_o[ROWS][PIECES][D];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int b = blockIdx.y;
+  const int n = fp4_len(p, fp4_sload(p.seq_lens + b));
+  if (n <= 0) return;
+  // where the request lies among all, and the spans that hold its tiles
+  const Fp4Plan plan = fp4_plan(p, lane);
+  const int span = fp4_span(plan.total, p.spans);
+  const int src = b / plan.per;
+  int start = __builtin_amdgcn_readlane(plan.before, src);
+  for (int x = src * plan.per; x < b; ++x) start += fp4_cost(fp4_len(p, fp4_sload(p.seq_lens + x)));
+  start += kFp4Begin;  // its first tile
+  const int first = start / span, pieces = (start + fp4_tiles(n) - 1) / span - first + 1;
   if (pieces <= 1) return;
-  for (int x = tid; x < b; x += 256) before += (dc_tiles_of(p.seq_lens[x]) + P - 1) / P;
-  const int first = dc_block_sum<256>(before, sm, tid);
-  const int part = tid / LANES, c = tid - part * LANES;
+  const int row = tid / (LANES * PIECES), part = tid / LANES % PIECES, c = tid % LANES;
+  const int rh = (int)blockIdx.x * ROWS + row;  // row of the request x head
+  const int j = rh / p.H, hd = rh - j * p.H;
+  const bool there = j < p.m && n - p.m + j >= 0;
   float top = kFp4MinusBig, sum = 0.f;
   f4_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int y = part; y < pieces; y += AT_ONCE) {
-    const int64_t slot = ((int64_t)(first + y) * p.m + j) * p.H + hd;
-    const float m1 = p.partial_ml[2 * slot], l1 = p.partial_ml[2 * slot + 1];
-    const f4_f32x4 o1 = *reinterpret_cast<const f4_f32x4*>(p.partial_o + slot * D + 4 * c);
-    const float m2 = fmaxf(top, m1);
-    const float fa = fp4_exp2(top - m2), fb = fp4_exp2(m1 - m2);
-    acc = acc * fa + o1 * fb;
-    sum = sum * fa + l1 * fb;
-    top = m2;
-  }
-  if (c == 0) sm_m[part] = top, sm_l[part] = sum;
-  *reinterpret_cast<f4_f32x4*>(&sm_o[part][4 * c]) = acc;
-  __syncthreads();
-  if (tid < D) {
-    float tm = kFp4MinusBig, tl = 0.f, x = 0.f;
-#pragma unroll
-    for (int y = 0; y < AT_ONCE; ++y) tm = fmaxf(tm, sm_m[y]);
-#pragma unroll
-    for (int y = 0; y < AT_ONCE; ++y) {
-      const float f = fp4_exp2(sm_m[y] - tm);
-      tl += sm_l[y] * f;
-      x += sm_o[y][tid] * f;
+  if (there) {
+#pragma unroll 4
+    for (int y = part; y < pieces; y += PIECES) {
+      const int64_t slot = ((int64_t)(first + y + b) * p.m + j) * p.H + hd;
+      const f4_f32x2 ml = *reinterpret_cast<const f4_f32x2*>(p.partial_ml + 2 * slot);
+      const f4_f32x4 o1 = *reinterpret_cast<const f4_f32x4*>(p.partial_o + slot * D + 4 * c);
+      const float m2 = fmaxf(top, ml[0]);
+      const float fa = fp4_exp2(top - m2), fb = fp4_exp2(ml[0] - m2);
+      acc = acc * fa + o1 * fb;
+      sum = sum * fa + ml[1] * fb;
+      top = m2;
     }
-    fp4_store_out(p.out, ((int64_t)b * p.m + j) * p.out_stride_t + hd * p.out_stride_h + tid, x / tl, p.out_f32 != 0, BF16);
+  }
+  if constexpr (PIECES > 1) {
+    if (c == 0) sm_ml[row][part][0] = top, sm_ml[row][part][1] = sum;
+    *reinterpret_cast<f4_f32x4*>(&sm_o[row][part][4 * c]) = acc;
+    __syncthreads();
+    if (part != 0) return;
+    float tm = kFp4MinusBig, tl = 0.f;
+    f4_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int y = 0; y < PIECES; ++y) tm = fmaxf(tm, sm_ml[row][y][0]);
+#pragma unroll
+    for (int y = 0; y < PIECES; ++y) {
+      const float f = fp4_exp2(sm_ml[row][y][0] - tm);
+      tl += sm_ml[row][y][1] * f;
+      x += *reinterpret_cast<const f4_f32x4*>(&sm_o[row][y][4 * c]) * f;
+    }
+    acc = x;
+    sum = tl;
+  }
+  if (there) {
+    const int64_t at = ((int64_t)b * p.m + j) * p.out_stride_t + hd * p.out_stride_h + 4 * c;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) fp4_store_out(p.out, at + y, acc[y] / sum, p.out_f32 != 0, BF16);
   }
 }
 
-// Workgroup slots of the chip for the plan: the workgroups that are resident together.
-static int fp4_plan_slots(int head_dim, int64_t rows, int cus) { return cus * fp4_wgs_per_cu(head_dim, (int)(rows > 64 ? 64 : rows)); }
+// Spans per unit: as many as there are workgroups resident together on the chip.
+static int fp4_row_groups(int64_t rows) { return (int)((rows + 31) / 32); }
+static int fp4_spans(int head_dim, int64_t rows, int kv_heads, int cus) {
+  return imax(1, cus * fp4_wgs_per_cu(head_dim, rows > 16 ? 32 : 16) / (kv_heads * fp4_row_groups(rows)));
+}
 
 static int fp4_cus(int* out) {
   static std::atomic<int> cache[64];
@@ -507,14 +704,23 @@ static int fp4_cus(int* out) {
 }
 
 template <int D, bool BF16>
-static void fp4_launch(const Fp4DecodeParams& p, int pieces, hipStream_t s) {
-  const unsigned grid = (unsigned)pieces * (unsigned)p.Hkv;
+static void fp4_launch(const Fp4DecodeParams& p, hipStream_t s) {
+  const unsigned grid = ((unsigned)p.spans * (unsigned)p.units + 7) / 8 * 8;
   const int R = p.m * p.G;
   if (R <= 8) fp4_decode_kernel<D, BF16, 1, true><<<grid, 256, 0, s>>>(p);
   else if (R <= 16) fp4_decode_kernel<D, BF16, 1, false><<<grid, 256, 0, s>>>(p);
-  else if (R <= 32) fp4_decode_kernel<D, BF16, 2, false><<<grid, 256, 0, s>>>(p);
-  else fp4_decode_kernel<D, BF16, 4, false><<<grid, 256, 0, s>>>(p);
-  fp4_join_kernel<D, BF16><<<dim3((unsigned)(p.m * p.H), (unsigned)p.batch), 256, 0, s>>>(p);
+  else fp4_decode_kernel<D, BF16, 2, false><<<grid, 256, 0, s>>>(p);
+  // pieces of a request that are joined side by side: as many as an average one can have
+  const unsigned rows = (unsigned)(p.m * p.H);
+  const int pieces = p.spans / p.batch;
+  auto join = [&](auto pieces_) {
+    constexpr int P = decltype(pieces_)::value;
+    constexpr unsigned threads = D / 4 * P < 256 ? 256 : D / 4 * P, per = threads / (D / 4 * P);
+    fp4_join_kernel<D, BF16, P><<<dim3((rows + per - 1) / per, (unsigned)p.batch), threads, 0, s>>>(p);
+  };
+  if (pieces < 4) join(std::integral_constant<int, 2>{});
+  else if (pieces < 24) join(std::integral_constant<int, 8>{});
+  else join(std::integral_constant<int, 32>{});
 }
 
 }  // namespace tmx
@@ -524,9 +730,7 @@ extern "C" int64_t tmx_decode_fp4_workspace_rows(int batch, int rows_per_request
   if (batch <= 0 || rows_per_request <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0) return 0;
   if (num_cus <= 0 && fp4_cus(&num_cus) != TMX_OK) return -1;
   const int64_t R = (int64_t)rows_per_request * (num_heads / num_kv_heads);
-  const int slots = fp4_plan_slots(head_dim, R, num_cus);
-  const int64_t pieces = (slots + num_kv_heads - 1) / num_kv_heads + (int64_t)batch;  // bound of the step's pieces
-  return pieces * rows_per_request * num_heads;
+  return (fp4_spans(head_dim, R > 64 ? 64 : R, num_kv_heads, num_cus) + (int64_t)batch) * rows_per_request * num_heads;
 }
 
 extern "C" int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* a, void* stream) {
@@ -566,21 +770,25 @@ extern "C" int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* a, void* st
   TMX_CHECK_ARG(a->q_stride_t >= 0 && a->q_stride_h >= 0 && a->q_stride_t % 8 == 0 && a->q_stride_h % 8 == 0 &&
                     a->out_stride_t >= 0 && a->out_stride_h >= 0,
                 "tmx_decode_attention_fp4: strides must not be negative, those of q multiples of 8 elements");
+  // tiles of a step are counted in 32 bits
+  const int64_t len_cap = (int64_t)a->max_blocks * a->page_size + a->rows_per_request;
+  TMX_CHECK_SUPPORTED(len_cap <= 0x7fffff00 && (len_cap / kBlockN + 2 + kFp4Begin) * a->batch <= 0x7fffff00,
+                      "tmx_decode_attention_fp4: the block table has room for more than 2^31 tiles of 32 keys");
   int cus = 0;
   {
     const int rc = fp4_cus(&cus);
     if (rc != TMX_OK) return rc;
   }
   Fp4DecodeParams p{};
-  p.plan_slots = fp4_plan_slots(a->head_dim, R, cus);
-  const int64_t pieces = (p.plan_slots + a->num_kv_heads - 1) / a->num_kv_heads + (int64_t)a->batch;
-  const int64_t rows = pieces * a->rows_per_request * a->num_heads;
+  p.spans = fp4_spans(a->head_dim, R, a->num_kv_heads, cus);
+  p.row_groups = fp4_row_groups(R);
+  p.units = a->num_kv_heads * p.row_groups;
+  const int64_t rows = (p.spans + (int64_t)a->batch) * a->rows_per_request * a->num_heads;
   TMX_CHECK_ARG(a->partial_o != nullptr && a->partial_ml != nullptr && ((uintptr_t)a->partial_o % 16 == 0),
                 "tmx_decode_attention_fp4: the work area is missing (tmx_decode_fp4_workspace_rows)");
   TMX_CHECK_ARG(a->workspace_rows >= rows,
                 "tmx_decode_attention_fp4: the work area holds %lld rows, this batch size needs %lld (tmx_decode_fp4_workspace_rows)",
                 (long long)a->workspace_rows, (long long)rows);
-  TMX_CHECK_SUPPORTED(pieces * a->num_kv_heads <= 0x7fffffff, "tmx_decode_attention_fp4: too many workgroups");
   p.q = a->q;
   p.out = a->out;
   p.k = (const uint8_t*)a->k;
@@ -592,6 +800,7 @@ extern "C" int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* a, void* st
   p.max_blocks = a->max_blocks;
   p.page_shift = __builtin_ctz(a->page_size);
   p.seq_lens = a->seq_lens;
+  p.len_cap = (int)len_cap;
   p.batch = a->batch;
   p.m = a->rows_per_request;
   p.H = a->num_heads;
@@ -608,11 +817,11 @@ extern "C" int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* a, void* st
   hipStream_t s = (hipStream_t)stream;
   const bool bf16 = a->io_dtype == TMX_BF16;
   if (a->head_dim == 128) {
-    if (bf16) fp4_launch<128, true>(p, (int)pieces, s);
-    else fp4_launch<128, false>(p, (int)pieces, s);
+    if (bf16) fp4_launch<128, true>(p, s);
+    else fp4_launch<128, false>(p, s);
   } else {
-    if (bf16) fp4_launch<64, true>(p, (int)pieces, s);
-    else fp4_launch<64, false>(p, (int)pieces, s);
+    if (bf16) fp4_launch<64, true>(p, s);
+    else fp4_launch<64, false>(p, s);
   }
   TMX_CHECK_HIP(hipGetLastError());
   return TMX_OK;
