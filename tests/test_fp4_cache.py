@@ -467,3 +467,126 @@ def test_refusals_on_the_gpu():
         a.update(bad)
         with pytest.raises(RuntimeError):
             ops.gather_dequant_kv_fp4(*b.caches, a["bt"], a["sl"], cu, 20, 20, a["dt"], out=a["out"])
+
+
+# ------------------------------------------------------------------------------------------------ the backend
+def test_backend_takes_the_mxfp4_cache_type():
+    from vllm_trianglemix_amd.backend import TriangleMixAttentionBackend as B
+    assert B.get_kv_cache_shape(11, 16, 8, 128, "mxfp4") == (2, 11, 16, 8, 68)
+    assert B.get_kv_cache_shape(11, 16, 8, 128) == (2, 11, 16, 8, 128)
+    impl = B.get_impl_cls()(32, 128, 0.1, 8, None, None, "mxfp4", None, "decoder", None, use_triangle=True)
+    assert impl.fp4_cache and not impl.fp8_cache
+    with pytest.raises(NotImplementedError):
+        B.get_impl_cls()(32, 128, 0.1, 8, None, None, "int4", None, "decoder", None)
+
+
+def _steps_metadata(builder, q_lens, seq_lens, table, slots, prompts=None):
+    import types
+    cu = np.concatenate([[0], np.cumsum(q_lens)]).astype(np.int32)
+    m = types.SimpleNamespace(
+        num_actual_tokens=int(cu[-1]), max_query_len=int(max(q_lens)), max_seq_len=int(max(seq_lens)),
+        query_start_loc=torch.from_numpy(cu).to(DEV), query_start_loc_cpu=torch.from_numpy(cu),
+        seq_lens=torch.tensor(seq_lens, dtype=torch.int32, device=DEV), seq_lens_cpu=torch.tensor(seq_lens, dtype=torch.int32),
+        block_table_tensor=table, slot_mapping=slots)
+    if prompts is not None:
+        m.prompt_lens_cpu = np.asarray(prompts, np.int32)
+    return builder.build(0, m)
+
+
+def test_which_steps_the_backend_reads_in_place():
+    import types
+    from vllm_trianglemix_amd.backend import TriangleMixAttentionImpl, TriangleMixAttentionMetadata
+    tri = TriangleMixAttentionImpl(32, 128, 0.1, 8, None, None, "mxfp4", None, "decoder", None, use_triangle=True)
+    causal = TriangleMixAttentionImpl(32, 128, 0.1, 8, None, None, "mxfp4", None, "decoder", None, use_triangle=False)
+
+    def md(q, s, uniform_decode=False, prompts=None):
+        cu = np.concatenate([[0], np.cumsum(q)]).astype(np.int32)
+        return TriangleMixAttentionMetadata(
+            num_actual_tokens=int(cu[-1]), max_query_len=int(max(q)), query_start_loc=None, max_seq_len=int(max(s)), seq_lens=None,
+            block_table=None, slot_mapping=None, query_start_loc_cpu=cu, seq_lens_cpu=np.asarray(s, np.int32), page_size=16,
+            uniform_decode=uniform_decode, prompt_lens_cpu=None if prompts is None else np.asarray(prompts, np.int32))
+
+    last = tri.pattern[2]
+    for impl in (tri, causal):
+        assert impl._fp4_rows_in_place(md([1, 1], [9, 5], True)) == 1
+        assert impl._fp4_rows_in_place(md([4, 4], [9, 5])) == 4
+        assert impl._fp4_rows_in_place(md([4, 3], [9, 5])) == 0
+        assert impl._fp4_rows_in_place(md([17, 17], [90, 50])) == 0  # 68 rows per K/V head
+    assert causal._fp4_rows_in_place(md([4, 4], [9, 5], prompts=[20, 5])) == 4
+    assert tri._fp4_rows_in_place(md([4, 4], [9, 5], prompts=[20, 5])) == 0  # a chunk of a prompt, not its end
+    narrow = TriangleMixAttentionImpl(32, 128, 0.1, 8, None, None, "mxfp4", None, "decoder", None, use_triangle=True, num_last_tokens=4)
+    assert last > 4 and narrow._fp4_rows_in_place(md([4, 4], [9, 5])) == 0 and narrow._fp4_rows_in_place(md([3, 3], [9, 5])) == 3
+
+
+@gpu
+@pytest.mark.parametrize("dtype, D, H, Hkv", [(torch.bfloat16, 128, 8, 2), (torch.float16, 64, 4, 2)])
+@pytest.mark.parametrize("use_triangle", [True, False])
+def test_backend_serves_prompts_chunks_decode_and_drafts_from_a_4_bit_cache(dtype, D, H, Hkv, use_triangle):
+    """Two prompts in one step, a third in two chunks, decode steps and a step of drafted rows out of one cache: every step against the formula over what the cache holds."""
+    import types
+    from oracle import trianglemix_oracle as orc
+    from parity_tolerance import assert_close
+    from vllm_trianglemix_amd.backend import TriangleMixAttentionBackend as B
+    rng = np.random.default_rng(5)
+    page, pages, gate = 16, 80, 64
+    si, sl, last = 4, 32, 16
+    impl = B.get_impl_cls()(H, D, D ** -0.5, Hkv, None, None, "mxfp4", None, "decoder", None, use_triangle=use_triangle,
+                            num_sink_tokens=si, sliding_window_size=sl, num_last_tokens=last, short_sequence_gate=gate)
+    builder = B.get_builder_cls()(types.SimpleNamespace(block_size=page), ["l0"], None, torch.device(DEV))
+    kv = torch.zeros(B.get_kv_cache_shape(pages, page, Hkv, D, "mxfp4"), dtype=torch.uint8, device=DEV)
+    order = rng.permutation(pages)
+    table = np.zeros((3, 24), np.int32)
+    for r in range(3):
+        table[r] = order[24 * r:24 * r + 24]
+    table_dev = torch.from_numpy(table).to(DEV)
+    lens, held = [0, 0, 0], [[np.zeros((0, Hkv, D)) for _ in range(2)] for _ in range(3)]
+
+    def step(q_lens, prompts=None, rows=None):
+        live = [r for r in range(3) if q_lens[r]]
+        ql = [q_lens[r] for r in live]
+        T = sum(ql)
+        q, k, v = (torch.from_numpy(rng.standard_normal((T, n, D))).to(dtype) for n in (H, Hkv, Hkv))
+        slots, at = [], 0
+        for r in live:
+            pos = np.arange(lens[r], lens[r] + q_lens[r])
+            slots.append(table[r, pos // page].astype(np.int64) * page + pos % page)
+            for x, new in enumerate((k, v)):
+                held[r][x] = np.concatenate([held[r][x], ref.values(*ref.quantise(new[at:at + q_lens[r]].double().numpy()))])
+            at += q_lens[r]
+            lens[r] += q_lens[r]
+        sls = [lens[r] for r in live]
+        m = _steps_metadata(builder, ql, sls, table_dev[live].contiguous(), torch.from_numpy(np.concatenate(slots)).to(DEV),
+                            None if prompts is None else [prompts[r] for r in live])
+        if rows is not None:
+            assert impl._fp4_rows_in_place(m) == rows
+        out = torch.zeros(T, H * D, dtype=dtype, device=DEV)
+        impl.forward(None, q.to(DEV).view(T, -1), k.to(DEV).view(T, -1), v.to(DEV).view(T, -1), kv, m, out)
+        cu = np.concatenate([[0], np.cumsum(ql)]).astype(np.int32)
+        got = out.view(T, H, D).double().cpu().numpy()
+        for i, r in enumerate(live):
+            n = sls[i]
+            full = n if prompts is None else max(n, prompts[r])
+            mode = "triangle" if use_triangle and full > gate else "causal"
+            kw = dict(full_lens=[full]) if full != n else {}
+            want = orc.varlen_gqa_attention(q[cu[i]:cu[i + 1]].double().numpy(), lambda b: held[r][0], lambda b: held[r][1],
+                                            [0, ql[i]], [n], D ** -0.5, mode, si, sl, last, **kw)
+            assert_close(got[cu[i]:cu[i + 1]], want, "backend forward, 4-bit cache", out16=True)
+
+    step([150, 40, 0], rows=0)
+    step([1, 1, 0], rows=1)
+    step([0, 0, 96], prompts=[0, 0, 200], rows=0)
+    step([0, 0, 104], prompts=[0, 0, 200])
+    step([1, 1, 1], rows=1)
+    step([4, 4, 4], rows=4)
+    step([1, 30, 2], rows=0)
+
+
+@gpu
+def test_backend_copies_blocks_of_all_layers():
+    from vllm_trianglemix_amd.backend import TriangleMixAttentionBackend as B
+    layers = [torch.randint(0, 256, B.get_kv_cache_shape(9, 16, 2, 64, "mxfp4"), dtype=torch.uint8, device=DEV) for _ in range(3)]
+    want = [x.clone() for x in layers]
+    B.copy_blocks(layers, torch.tensor([[1, 4], [1, 5], [2, 0]]))
+    for x, y in zip(layers, want):
+        y[:, [4, 5, 0]] = y[:, [1, 1, 2]]
+        assert torch.equal(x, y)

@@ -171,6 +171,23 @@ class TriangleMixAttentionMetadata:
             self.__dict__["_whole_prompts"] = w
         return w
 
+    @property
+    def uniform_rows(self) -> int:
+        """Query rows per request when every request of the step has the same number of them, 0 otherwise."""
+        m = self.__dict__.get("_uniform_rows")
+        if m is None:
+            q = np.diff(self.query_start_loc_cpu)
+            same = q.shape[0] == self.seq_lens_cpu.shape[0] > 0 and bool(np.all(q == q[0]))
+            m = int(q[0]) if same and int(self.query_start_loc_cpu[-1]) == self.num_actual_tokens else 0
+            self.__dict__["_uniform_rows"] = m
+        return m
+
+    @property
+    def prompts_complete(self) -> bool:
+        """False while a request of the step is known to have more prompt to come (its last rows here are not the last
+        rows of its pattern)."""
+        return self.prompt_lens_cpu is None or bool(np.all(self.prompt_lens_cpu <= self.seq_lens_cpu))
+
     def fp8_row_offsets(self, device):
         """Row offsets of every request's keys in a contiguous copy of the step's K/V (``cu_seqlens_k``), on the
         device, and their total: made once per step, shared by the layers."""
@@ -253,6 +270,14 @@ class TriangleMixMetadataBuilder(_BuilderBase):
         ws = self._decode_ws.get(key)
         if ws is None:
             ws = self._decode_ws[key] = ops.decode_workspace(batch, num_heads, num_kv_heads, head_size, self.device, fp8)
+        return ws
+
+    def decode_fp4_workspace(self, batch: int, rows: int, num_heads: int, num_kv_heads: int, head_size: int) -> tuple:
+        """The same for the launch that reads a 4-bit cache, per batch size and rows per request."""
+        key = ("fp4", batch, rows, num_heads, num_kv_heads, head_size)
+        ws = self._decode_ws.get(key)
+        if ws is None:
+            ws = self._decode_ws[key] = ops.decode_fp4_workspace(batch, rows, num_heads, num_kv_heads, head_size, self.device)
         return ws
 
     def build(self, common_prefix_len: int, common_attn_metadata, fast_build: bool = False
@@ -339,7 +364,17 @@ class TriangleMixAttentionBackend(_BackendBase):
         # same layout as rocm_attn.py:173-181; pages must be a power of two of at least 16 tokens
         if block_size < 16 or block_size & (block_size - 1):
             raise ValueError("Block size must be a power of two of at least 16.")
+        if cache_dtype_str == "mxfp4":
+            # 4-bit pages of uint8: codes and scale bytes, D / 2 + D / 32 bytes per token and head
+            return (2, *ops.fp4_cache_shape(num_blocks, block_size, num_kv_heads, head_size))
         return (2, num_blocks, block_size, num_kv_heads, head_size)
+
+    @staticmethod
+    def copy_blocks(kv_caches: List[torch.Tensor], src_to_dists: torch.Tensor) -> None:
+        """Pages ``src_to_dists[:, 0]`` of every layer's cache ``[2, num_blocks, ...]`` to pages ``src_to_dists[:, 1]``
+        (the reference's csrc/cache_kernels.cu copy_blocks), K and V of all layers in one launch."""
+        ops.copy_pages([kv for cache in kv_caches for kv in cache.unbind(0)],
+                       src_to_dists.to(kv_caches[0].device).contiguous() if len(kv_caches) else src_to_dists)
 
     @staticmethod
     def use_cascade_attention(*args, **kwargs) -> bool:
@@ -379,10 +414,11 @@ class TriangleMixAttentionImpl(_ImplBase):
                                       "(the TriangleMix pattern carries its own window)")
         if logits_soft_cap:
             raise NotImplementedError("logits soft cap is not supported by TriangleMixAttentionImpl")
-        if kv_cache_dtype not in ("auto", "bfloat16", "float16", "half", "fp8", "fp8_e4m3"):
+        if kv_cache_dtype not in ("auto", "bfloat16", "float16", "half", "fp8", "fp8_e4m3", "mxfp4"):
             raise NotImplementedError(f"kv_cache_dtype '{kv_cache_dtype}' is not supported "
-                                      "(16-bit caches and fp8 e4m3 are)")
+                                      "(16-bit caches, fp8 e4m3 and mxfp4 are)")
         self.fp8_cache = kv_cache_dtype.startswith("fp8")
+        self.fp4_cache = kv_cache_dtype == "mxfp4"
 
         cfg = trianglemix_config
         if cfg is None:
@@ -420,6 +456,8 @@ class TriangleMixAttentionImpl(_ImplBase):
         q = query.view(-1, self.num_heads, self.head_size)[:n_tok]
         if self.fp8_cache:
             return self._forward_fp8_cache(layer, q, key, value, key_cache, value_cache, m, output)
+        if self.fp4_cache:
+            return self._forward_fp4_cache(q, key, value, key_cache, value_cache, m, output)
         writes_cache = self.kv_sharing_target_layer_name is None and key is not None and value is not None
         out = output.view(-1, self.num_heads, self.head_size)[:n_tok]
         if m.uniform_decode and self._decode_fixed_ok():
@@ -542,3 +580,51 @@ class TriangleMixAttentionImpl(_ImplBase):
         ops.attention(q, k_rows, v_rows, out, idx, m.query_start_loc, m.seq_lens, self.scale, cu_seqlens_k=cu_k,
                       workspace=ws, flags=_step_flags(m))
         return output
+
+    def _forward_fp4_cache(self, q, key, value, key_cache, value_cache, m, output):
+        """kv_cache_dtype "mxfp4": the step's rows are quantised into the pages, and the attention reads what the pages
+        hold -- in place for steps whose requests all have the same few rows (decode, drafted tokens), through 16-bit
+        rows read back for the step otherwise (prompts)."""
+        n_tok = m.num_actual_tokens
+        out = output.view(-1, self.num_heads, self.head_size)[:n_tok]
+        if n_tok == 0:
+            return output
+        if self.kv_sharing_target_layer_name is None and key is not None and value is not None:
+            ops.reshape_and_cache_fp4(key[:n_tok].view(n_tok, self.num_kv_heads, self.head_size),
+                                      value[:n_tok].view(n_tok, self.num_kv_heads, self.head_size), key_cache, value_cache,
+                                      m.slot_mapping[:n_tok])
+        rows = self._fp4_rows_in_place(m)
+        if rows:
+            batch = n_tok // rows
+            if m.builder is not None:
+                ws = m.builder.decode_fp4_workspace(batch, rows, self.num_heads, self.num_kv_heads, self.head_size)
+            else:
+                ws = ops.decode_fp4_workspace(batch, rows, self.num_heads, self.num_kv_heads, self.head_size, q.device)
+            ops.decode_attention_fp4(q, key_cache, value_cache, out, m.block_table, m.seq_lens, self.scale, ws,
+                                     rows_per_request=rows)
+            return output
+        if m.capturing:
+            raise NotImplementedError("this layer has no decode launch that replays under a graph (num_last_tokens >= 2)")
+        mode = "triangle" if self.use_triangle else "causal"
+        pattern = self.pattern if self.use_triangle else (0, 0, 0)
+        tri_min_len = self.tri_min_len if self.use_triangle else 0
+        idx = m.block_index(mode, pattern, self.num_heads, self.num_kv_heads, tri_min_len, dense_kernel=self._dense_kernel_ok())
+        ws = m.workspace(idx, self.num_heads, self.head_size, q.device, self.num_kv_heads)
+        cu_k, total = m.fp8_row_offsets(q.device)
+        k_rows, v_rows = ops.gather_dequant_kv_fp4(key_cache, value_cache, m.block_table, m.seq_lens, cu_k, total,
+                                                   int(m.max_seq_len), q.dtype)
+        ops.attention(q, k_rows, v_rows, out, idx, m.query_start_loc, m.seq_lens, self.scale, cu_seqlens_k=cu_k,
+                      workspace=ws, flags=_step_flags(m))
+        return output
+
+    def _fp4_rows_in_place(self, m) -> int:
+        """Rows per request of a step that the in-place launch covers, 0 for others.  It attends to every key up to a
+        row's position: any causal layer's rows, and a triangle layer's when they all lie among the trailing dense rows
+        (row i of a sequence of N: N - i < last, trianglemix_attention.py:126-129).  A decode step is taken as one whatever
+        its prompts' lengths, as with the other caches."""
+        rows = 1 if m.uniform_decode else m.uniform_rows
+        if rows < 1 or rows * (self.num_heads // self.num_kv_heads) > 64 or (rows == 1 and not m.uniform_decode):
+            return 0
+        if self.use_triangle and (self.pattern[2] <= rows or (rows > 1 and not m.prompts_complete)):
+            return 0
+        return rows

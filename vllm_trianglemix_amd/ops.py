@@ -816,7 +816,7 @@ def _fp4_caches(key_cache: torch.Tensor, value_cache: torch.Tensor) -> int:
 def _call(op, *args):
     """A registered operator's call: its refusals come as TmxError, like the library's own."""
     try:
-        return op(*args)
+        return op.default(*args)
     except (RuntimeError, NotImplementedError) as e:
         raise _lib.TmxError(-1, str(e)) from None
 
