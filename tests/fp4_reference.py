@@ -61,11 +61,11 @@ def unpack(raw, heads, dim, page, is_v):
 
 
 def attention(q, k, v, scale, m):
-    """Rows ``q [m, H, D]`` at the last m positions of keys ``k / v [n, Hkv, D]``: outputs, sum p |v|, and the largest
-    sum |q k| scale of a row (what the scores' rounding errors are proportional to).  Rows at negative positions: NaN."""
+    """Rows ``q [m, H, D]`` at the last m positions of keys ``k / v [n, Hkv, D]``: outputs, sum p |v|, and a bound of the
+    error of a row's scores (see :func:`bound`).  Rows at negative positions: NaN."""
     n, hkv, dim = k.shape
     H = q.shape[1]
-    o, av, qk = (np.full((m, H, dim), np.nan) for _ in range(3))
+    o, av, ds = (np.full((m, H, dim), np.nan) for _ in range(3))
     for j in range(m):
         seen = n - m + 1 + j
         if seen <= 0:
@@ -77,14 +77,18 @@ def attention(q, k, v, scale, m):
                 p = np.exp(s - s.max())
                 p /= p.sum()
                 o[j, h], av[j, h] = p @ vv, p @ np.abs(vv)
-                qk[j, h] = (np.abs(kk) @ np.abs(q[j, h])).max() * scale
-    return o, av, qk
+                ds[j, h] = scale * (dim + 8) * 2.0 ** -23 * (np.abs(kk) @ np.abs(q[j, h])).max()
+    return o, av, ds
 
 
-def bound(o, av, qk, n, dim, half_step):
-    """Error bound of an output.  half_step |o|: its own rounding.  Times sum p |v|: the probabilities' two bf16 terms
-    (2^-16), fp32 sums over n keys (each wave's accumulator adds a product of 32 keys every 128 keys; the sum over its
-    pieces; 2^-23 each) and the scores' error: an fp32 sum of dim exact products, twice because numerator and denominator
-    both carry it."""
-    gamma = 2.0 ** -16 + (n / 64 + 64) * 2.0 ** -23 + 2 * (dim + 8) * 2.0 ** -23 * qk
+def bound(o, av, ds, n, half_step):
+    """Error bound of an output.
+
+    half_step |o|: its own rounding.  Times sum p |v|: the probabilities' two bf16 terms (2^-16), fp32 sums over n keys
+    (each wave's accumulator adds a product of 32 keys every 128 keys; the sum over its pieces; 2^-23 each), and the
+    scores' error ds: with scores off by at most ds every weight p_j / sum p is off by a factor between exp(-2 ds) and
+    exp(2 ds), so the output by at most (exp(2 ds) - 1) sum p |v|.  ds is the rounding of an fp32 sum of dim
+    exact products, (dim + 8) 2^-23 sum |q k|."""
+    with np.errstate(over="ignore"):
+        gamma = 2.0 ** -16 + (n / 64 + 64) * 2.0 ** -23 + np.expm1(2 * ds)
     return half_step * np.abs(o) + gamma * av + 1e-30

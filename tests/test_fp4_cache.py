@@ -80,11 +80,15 @@ def _args(**kw):
     (dict(kv_stride_page=16 * 2 * 68 - 16), _lib.TMX_ERR_INVALID_ARG), (dict(kv_stride_page=16 * 2 * 68 + 8), _lib.TMX_ERR_INVALID_ARG),
     (dict(k=4104), _lib.TMX_ERR_INVALID_ARG), (dict(q_stride_h=132), _lib.TMX_ERR_INVALID_ARG),
     (dict(max_blocks=-1), _lib.TMX_ERR_INVALID_ARG), (dict(batch=-1), _lib.TMX_ERR_INVALID_ARG),
-    (dict(batch=70000), _lib.TMX_ERR_UNSUPPORTED),
+    (dict(batch=70000), _lib.TMX_ERR_UNSUPPORTED), (dict(num_heads=2048, num_kv_heads=1024, page_size=1 << 20), _lib.TMX_ERR_UNSUPPORTED),
+    (dict(max_blocks=2 ** 31 - 1), _lib.TMX_ERR_UNSUPPORTED), (dict(batch=60000, max_blocks=1 << 20), _lib.TMX_ERR_UNSUPPORTED),
+    (dict(workspace_rows=1 << 4), None),
 ])
 def test_decode_refuses_bad_arguments(change, code):
     lib = _lib.load()
-    assert lib.tmx_decode_attention_fp4(ctypes.byref(_args(**change)), None) == code
+    got = lib.tmx_decode_attention_fp4(ctypes.byref(_args(**change)), None)
+    # (too small a work area shows once the chip's size is known; without a chip that is an error of its own)
+    assert got == code if code is not None else got in (_lib.TMX_ERR_INVALID_ARG, _lib.TMX_ERR_HIP)
     assert lib.tmx_last_error()
 
 
@@ -248,12 +252,13 @@ class Batch:
             if n <= 0:
                 assert (got[rows] == 7).all()
                 continue
-            o, av, qk = ref.attention(qd[rows], *self.keys(b), self.scale, self.m)
+            o, av, ds = ref.attention(qd[rows], *self.keys(b), self.scale, self.m)
             there = np.arange(self.m) >= self.m - n
             assert (got[rows][~there] == 7).all()
-            lim = ref.bound(o, av, qk, n, self.D, HALF[out_dtype or dtype])[there]
+            lim = ref.bound(o, av, ds, n, HALF[out_dtype or dtype])[there]
             err = np.abs(got[rows][there] - o[there])
-            assert (err <= lim).all(), (b, n, float((err / lim).max()))
+            worst = float((err / lim).max())
+            assert worst <= 1, (b, n, worst)
 
 
 @gpu
@@ -279,6 +284,17 @@ def test_decode_head_layouts(heads, kv_heads, dtype):
 def test_several_rows_per_request(m, dtype, dim):
     """Lengths below, at and above the number of rows; rows before the sequence's start are left alone."""
     Batch(m, [m - 1, m, m + 1, 1, 0, 32, 33, 47, 64 + m, 500], 8, 2, dim, 16, m=m).check(dtype)
+
+
+@gpu
+@pytest.mark.parametrize("batch", [64, 65, 130])
+def test_many_requests(batch):
+    """More requests than lanes that count them; empty ones among them, one that is much longer than the others."""
+    rng = np.random.default_rng(batch)
+    lens = [int(n) for n in rng.integers(-2, 90, batch)]
+    lens[1], lens[batch // 2], lens[-1] = 0, 2000, 33
+    Batch(batch, lens, 4, 1, 64, 16, m=2).check(torch.bfloat16)
+    Batch(batch + 1, [0] * (batch - 1) + [5], 4, 2, 128, 16).check(torch.float16)
 
 
 @gpu
@@ -339,6 +355,53 @@ def test_a_nan_reaches_the_rows_that_see_it_and_no_other(dim, dtype):
             hit[2:4, 4:8] = True
         assert torch.equal(nan, hit)
         assert torch.equal(got[~hit], want[~hit])
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_query_that_is_not_finite_spoils_its_own_row_only(dim, dtype):
+    for heads, m in ((8, 1), (8, 3), (32, 2)):
+        b = Batch(16, [70, 33], heads, 2, dim, 16, m=m)
+        _, want = b.run(dtype)
+        b.q[0, 1, 5], b.q[1, heads - 1, dim - 1], b.q[m, 3, 0] = np.nan, np.inf, -np.inf
+        _, got = b.run(dtype)
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[0, 1], hit[1, heads - 1], hit[m, 3] = True, True, True
+        assert torch.equal(torch.isnan(got), hit) and torch.equal(got[~hit], want[~hit])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_queries_and_keys_of_very_different_sizes(dtype):
+    """Neighbouring query columns that differ by up to 2^19, keys scaled block by block: every product has to count in the
+    scores as it does in an fp32 sum."""
+    rng = np.random.default_rng(17)
+    b = Batch(17, [300, 45, 1025], 8, 2, 128, 32, m=2)
+    b.q *= np.ldexp(1.0, rng.integers(-13, 7, b.q.shape))
+    for x in (0, 1):
+        nb = b.Hkv * b.page * b.D // 2
+        shift = rng.integers(-9, 5, b.raw[x][:, nb:].shape)
+        b.raw[x][:, nb:] = np.clip(b.raw[x][:, nb:].astype(int) + shift, 1, 253).astype(np.uint8)
+        b.caches[x].copy_(torch.from_numpy(b.raw[x]).to(DEV).view(b.caches[x].shape))
+    b.scale = 0.01
+    b.check(dtype, torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("seed", range(40))
+def test_random_steps(seed):
+    rng = np.random.default_rng(1000 + seed)
+    kv = int(rng.choice([1, 2, 3, 4, 5, 8]))
+    group = int(rng.integers(1, 17))
+    m = int(rng.integers(1, max(2, min(9, 64 // group + 1))))
+    batch = int(rng.choice([1, 2, 3, 7, 20]))
+    lens = [int(n) for n in np.exp(rng.uniform(0, np.log(1500), batch)).astype(int)]
+    if batch > 2:
+        lens[int(rng.integers(batch))] = int(rng.integers(-1, 3))
+    b = Batch(seed, lens, kv * group, kv, int(rng.choice([64, 128])), int(rng.choice([16, 32, 64, 256])), m=m,
+              page_gap=int(rng.choice([0, 16, 80])))
+    b.check([torch.bfloat16, torch.float16][seed % 2], [None, torch.float32][seed // 2 % 2])
 
 
 @gpu

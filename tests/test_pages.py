@@ -330,8 +330,8 @@ def test_a_serving_run(dtype):
             ops.decode_attention_fp4(q.to(DEV), kc[x], vc[x], out, table[live].contiguous(), t32([lens[s] for s in live]), D ** -0.5,
                                      ops.decode_fp4_workspace(len(live), m, H, Hkv, D, DEV), rows_per_request=m)
             for i, s in enumerate(live):
-                o, av, qk = ref.attention(q[i * m:(i + 1) * m].double().numpy(), *kept[s][x], D ** -0.5, m)
-                assert (np.abs(out[i * m:(i + 1) * m].double().cpu().numpy() - o) <= ref.bound(o, av, qk, lens[s], D, 2.0 ** -24)).all(), (s, x)
+                o, av, ds = ref.attention(q[i * m:(i + 1) * m].double().numpy(), *kept[s][x], D ** -0.5, m)
+                assert (np.abs(out[i * m:(i + 1) * m].double().cpu().numpy() - o) <= ref.bound(o, av, ds, lens[s], 2.0 ** -24)).all(), (s, x)
 
     def start(row):
         nonlocal table

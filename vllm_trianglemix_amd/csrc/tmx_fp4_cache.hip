@@ -146,7 +146,8 @@ static int fp4_check_cache(const char* fn, const void* k, const void* v, int64_t
   TMX_CHECK_SUPPORTED(page_size >= 16 && page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0,
                       "%s: page_size %d not supported (powers of two from 16 to 2^20 are)", fn, page_size);
   TMX_CHECK_SUPPORTED(num_pages <= 0x7fffffff, "%s: more than 2^31 - 1 pages", fn);
-  TMX_CHECK_SUPPORTED(kv_heads <= 1024, "%s: more than 1024 K/V heads", fn);
+  TMX_CHECK_SUPPORTED(kv_heads <= 1024 && fp4_page_bytes(kv_heads, page_size, head_dim) <= 0x7fffffff,
+                      "%s: more than 1024 K/V heads, or a page of 2^31 bytes or more", fn);
   TMX_CHECK_ARG(stride_page >= fp4_page_bytes(kv_heads, page_size, head_dim) && stride_page % 16 == 0,
                 "%s: the page stride %lld must be a multiple of 16 bytes and hold a page of %lld", fn, (long long)stride_page,
                 (long long)fp4_page_bytes(kv_heads, page_size, head_dim));

@@ -6,14 +6,15 @@
 //   workgroup = 4 waves = a span of 32-key tiles x one K/V head; the waves take the span's tiles in turn and meet only at
 //   a request's end.  Rows = rows_per_request x (query heads per K/V head), all of them columns of the same products, so
 //   a head's K/V are read once whatever the group size.
-//   Scores S^T = K Q^T: K goes to the matrix cores as it lies in the cache (v_mfma_scale_f32_16x16x128_f8f6f4, 4-bit
-//   operand, one scale byte per key and 32 columns), nothing is converted.  Q^T is the 8-bit operand, split into two terms
-//   of 4 significant bits (bf16 queries: 8 bits) or three (fp16: 11), each with a power of two per 32 columns: the terms
-//   hold every query value down to 2^-14 of its block's largest exactly and smaller ones to 2^-22 (bf16; fp16 2^-26) of it,
-//   below the rounding of the fp32 sums.  Row m of product t is key 16 t + m of the tile.
-//   Output O^T = V^T P^T (v_mfma_f32_16x16x32_bf16): lane (m = lane % 16, g = lane / 16) needs columns [m D/16, (m + 1)
+//   Scores S^T = K Q^T (v_mfma_f32_16x16x32_bf16, D / 32 of them per 16 keys): lane (m = lane % 16, g = lane / 16) holds
+//   columns [g D/4, (g + 1) D/4) of key row m, one load and one scale; the codes become bf16, which is exact (one fraction
+//   bit, power-of-two scales).  The head dimension may be summed in any order as long as Q^T is laid out alike.  fp16
+//   queries are split into two bf16 terms (exact: 11 bits in 8 + 8).  (The scaled product that takes 4-bit operands as
+//   they are would save these conversions, but it sums 8 neighbouring products with some 14 bits below the largest of
+//   them: a query column 2^7 below its neighbours would not count.)
+//   Output O^T = V^T P^T (the same product): lane (m, g) needs columns [m D/16, (m + 1)
 //   D/16) of the 8 keys whose scores it holds, 4 g .. 4 g + 3 and 16 + 4 g .. + 3.  The cache keeps V in that order
-//   (tmx_fp4.h), so V comes straight from memory, becomes bf16 (exact: one fraction bit, power-of-two scales) by 32
+//   (tmx_fp4.h), so V comes straight from memory, becomes bf16 by 32
 //   conversions and is paired by 32 byte permutes; the probabilities never leave their lane.  No LDS in the loop.
 //   Probabilities are held as two bf16 terms (16 significant bits; one term alone would cost as much accuracy as the
 //   rounding of the output).  Up to 8 rows, columns 8..15 repeat the rows and carry the second term: no extra product.
@@ -31,9 +32,6 @@ namespace tmx {
 typedef __attribute__((ext_vector_type(4))) float f4_f32x4;
 typedef __attribute__((ext_vector_type(8))) __bf16 f4_bf16x8;
 typedef __attribute__((ext_vector_type(2))) float f4_f32x2;
-typedef __attribute__((ext_vector_type(8))) int f4_i32x8;
-typedef __attribute__((ext_vector_type(2))) unsigned short f4_u16x2;
-typedef __attribute__((ext_vector_type(2))) short f4_s16x2;
 
 constexpr float kFp4MinusBig = -3.0e38f;  // below every finite score, and finite
 constexpr float kFp4Slack = 8.0f;
@@ -85,7 +83,7 @@ __device__ __forceinline__ void fp4_store_out(void* out, int64_t at, float x, bo
 // change over (queries split anew, the waves' sums joined and written).  A span may begin and end inside requests: piece
 // (span w, request b) of a request that lies in several spans leaves its result in slot w + b -- both only grow along the
 // tiles, so no two pieces share a slot -- and the pieces are joined afterwards.  Every wave works the plan out for itself, without a barrier: lane l
-// counts the tiles of a run of requests, six shuffles sum the lanes. ----
+// counts the tiles of a run of requests, six lane moves sum them up. ----
 constexpr int kFp4MinSpan = 4;  // a tile per wave
 constexpr int kFp4Begin = 12;
 __device__ __forceinline__ int fp4_len(const Fp4DecodeParams& p, int n) { return imin(n, p.len_cap); }
@@ -97,23 +95,34 @@ __device__ __forceinline__ int fp4_span(int tiles, int spans) {
 }
 struct Fp4Plan {
   int per;                  // requests per lane
+  int len;                  // the last one's length (per == 1: lane b holds request b's)
   int mine, before, total;  // cost of this lane's requests, of those before them, of all
 };
 __device__ __forceinline__ Fp4Plan fp4_plan(const Fp4DecodeParams& p, int lane) {
   Fp4Plan r;
   r.per = (p.batch + 63) >> 6;
   const int j0 = imin(p.batch, lane * r.per), j1 = imin(p.batch, j0 + r.per);
-  r.mine = 0;
-  for (int j = j0; j < j1; ++j) r.mine += fp4_cost(fp4_len(p, p.seq_lens[j]));
-  int inc = r.mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int up = __shfl_up(inc, d, 64);
-    if (lane >= d) inc += up;
+  r.mine = r.len = 0;
+  for (int j = j0; j < j1; ++j) {
+    r.len = fp4_len(p, p.seq_lens[j]);
+    r.mine += fp4_cost(r.len);
   }
+  // inclusive sum over the lanes: within rows of 16, then the rows' totals down the wave
+  int inc = r.mine;
+  inc += __builtin_amdgcn_update_dpp(0, inc, 0x111, 0xf, 0xf, false);  // row_shr:1
+  inc += __builtin_amdgcn_update_dpp(0, inc, 0x112, 0xf, 0xf, false);  // row_shr:2
+  inc += __builtin_amdgcn_update_dpp(0, inc, 0x114, 0xf, 0xf, false);  // row_shr:4
+  inc += __builtin_amdgcn_update_dpp(0, inc, 0x118, 0xf, 0xf, false);  // row_shr:8
+  inc += __builtin_amdgcn_update_dpp(0, inc, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  inc += __builtin_amdgcn_update_dpp(0, inc, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
   r.before = inc - r.mine;
   r.total = __builtin_amdgcn_readlane(inc, 63);
   return r;
+}
+
+// request b's length (uniform): from the lane that counted it, or from memory
+__device__ __forceinline__ int fp4_len_of(const Fp4DecodeParams& p, const Fp4Plan& plan, int b) {
+  return plan.per == 1 ? __builtin_amdgcn_readlane(plan.len, b) : fp4_len(p, fp4_sload(p.seq_lens + b));
 }
 
 // Workgroups resident per CU.  Two per CU with a tile read ahead per wave have 70 KB in flight, all that the memory
@@ -127,9 +136,8 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
   static_assert(!HALF || NT == 1, "the half form has one tile");
   constexpr int DT = D / 16;        // row tiles of the second product
   constexpr int VW = D / 32;        // words of V codes per lane and page-half
-  constexpr int TERMS = BF16 ? 2 : 3;
-  // D = 64 fills half of the product's 128 columns: two terms share one product (K twice, the terms side by side)
-  constexpr int PRODUCTS = D == 128 ? TERMS : (TERMS + 1) / 2;
+  constexpr int KS = D / 32;        // k-steps of the first product
+  constexpr int TERMS = BF16 ? 1 : 2;  // of the query
   constexpr int ROWS = HALF ? 8 : 16 * NT;
   __shared__ __attribute__((aligned(16))) float sm_o[4][ROWS][D + 4];  // (+ 4: the rows a wave writes at once start in different banks)
   __shared__ f4_f32x2 sm_ml[4][ROWS];
@@ -147,8 +155,8 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
 
   // the request at which this workgroup's span begins, and where in it
   int b, off, left;
+  const Fp4Plan plan = fp4_plan(p, lane);
   {
-    const Fp4Plan plan = fp4_plan(p, lane);
     const int span = fp4_span(plan.total, p.spans);
     const long long begin_ = (long long)w * span;
     if (begin_ >= plan.total) return;  // fewer spans in this step than the grid provides for
@@ -158,7 +166,7 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
     b = src * plan.per;
     int at = __builtin_amdgcn_readlane(plan.before, src);
     for (;;) {
-      const int cj = fp4_cost(fp4_len(p, fp4_sload(p.seq_lens + b)));
+      const int cj = fp4_cost(fp4_len_of(p, plan, b));
       if (begin < at + cj) break;
       at += cj;
       ++b;
@@ -171,13 +179,13 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
   const int64_t head_codes = (int64_t)h * ps * (D / 2);
   const int scales_from_codes = (int)(fp4_code_bytes(p.Hkv, ps, D) + (int64_t)h * ps * (D / 32) - head_codes);
   // byte offsets of a lane inside a page-half of a head
-  const int k_lane = c16 * (D / 2) + (D == 128 ? g : g & 1) * 16;
+  const int k_lane = c16 * (D / 2) + g * (D / 8);
   const int v_lane = D == 128 ? g * 256 + c16 * 16 : (g >> 1) * 256 + c16 * 16 + (g & 1) * 8;
-  const int ks_lane = (D == 128 ? g : g & 1) * ps + c16;
+  const int ks_lane = (D == 128 ? g : g >> 1) * ps + c16;
   const int vs_lane = (D == 128 ? c16 >> 2 : c16 >> 3) * ps + 4 * g;
 
   struct Raw {
-    fp4_u32x4 k[2];                  // 32 codes of key 16 t + c16
+    unsigned k[2][KS];               // D / 4 codes of key 16 x + c16
     unsigned v[2 * VW];              // codes of keys 4 g .. + 3 and 16 + 4 g .. + 3, D / 16 columns each
     unsigned ks[2];                  // scale bytes
     unsigned vs[2];                  // four keys' scale bytes each
@@ -217,12 +225,17 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
       const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.k) + base, 0, 0x7fffffff, 0x00020000);
       const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.v) + base, 0, 0x7fffffff, 0x00020000);
       constexpr int kStream = 2;  // codes are read once: non-temporal (96 against 112 us for the loads of 64 x 8192)
-      r.k[x] = __builtin_bit_cast(fp4_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_lane, 0, kStream));
       if constexpr (D == 128) {
+        const fp4_u32x4 z = __builtin_bit_cast(fp4_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_lane, 0, kStream));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.k[x][i] = z[i];
         const fp4_u32x4 y = __builtin_bit_cast(fp4_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, v_lane, 0, kStream));
 #pragma unroll
         for (int i = 0; i < 4; ++i) r.v[4 * x + i] = y[i];
       } else {
+        const fp4_u32x2 z = __builtin_bit_cast(fp4_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rk, k_lane, 0, kStream));
+        r.k[x][0] = z[0];
+        r.k[x][1] = z[1];
         const fp4_u32x2 y = __builtin_bit_cast(fp4_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, v_lane, 0, kStream));
         r.v[2 * x] = y[0];
         r.v[2 * x + 1] = y[1];
@@ -231,8 +244,8 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
       r.vs[x] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rv, vs_lane, scales, 0);
     }
   };
-  // Lane column c16 = query row; the 8-bit operand of the product holds columns 16 g .. + 15 and 64 + 16 g .. + 15 of it.
-  // Row r is position n - m + r / G, head h G + r % G.
+  // Query rows: lane column c16 = row, k-step i covers columns g D/4 + 8 i .. + 7.  Row r is position n - m + r / G, head
+  // h G + r % G.
   auto load_q = [&]() {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -241,12 +254,12 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
       const int j = r / p.G, hd = h * p.G + (r - j * p.G);
       const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + ((int64_t)b * p.m + j) * p.q_stride_t + hd * p.q_stride_h;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) qraw[t][i] = *reinterpret_cast<const uint4*>(src + 64 * (i >> 1) + 16 * g + 8 * (i & 1));
+      for (int i = 0; i < D / 32; ++i) qraw[t][i] = *reinterpret_cast<const uint4*>(src + g * (D / 4) + 8 * i);
     }
   };
   // The next piece of the span: its query rows and first tiles are asked for here, before the one that ends is written out.
   auto start = [&]() {
-    n = fp4_len(p, fp4_sload(p.seq_lens + b));
+    n = fp4_len_of(p, plan, b);
     const int tiles = fp4_tiles(n), take = imin(left, tiles - off);
     left -= take;
     tile_end = off + take;
@@ -267,92 +280,31 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
   start();
   for (;;) {
     if constexpr (!QAHEAD) load_q();
-    // ---- the query's terms: x = 2^E (t0 + t1 / 16 + t2 / 256), E such that the block's largest lies in [128, 256) 2^E ----
-    f4_i32x8 qt[NT][PRODUCTS];
-    int qs[NT][PRODUCTS];  // scale bytes: lane (c16, g) gives the one of columns 32 g .. of the product
-    int pos[NT];           // the position of this lane's row
+    uint4 qt[NT][TERMS][KS];
+    int pos[NT];  // the position of this lane's row
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int row = HALF ? (c16 & 7) : 16 * t + c16;
       pos[t] = n - p.m + (row0 + (row < R ? row : 0)) / p.G;
-      unsigned w[D / 8];  // two columns each
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) w[4 * i] = qraw[t][i].x, w[4 * i + 1] = qraw[t][i].y, w[4 * i + 2] = qraw[t][i].z, w[4 * i + 3] = qraw[t][i].w;
-      int E[D / 64];
-      bool bad = false;
-#pragma unroll
-      for (int y = 0; y < D / 64; ++y) {
-        f4_u16x2 top = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(f4_u16x2, w[8 * y + i] & 0x7fff7fffu));
-        unsigned m = max((unsigned)top[0], (unsigned)top[1]);
-        m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));  // the block's other 16 columns
-        bad |= m >= (BF16 ? 0x7f80u : 0x7c00u);
-        const unsigned bits = BF16 ? m << 16 : __float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)m));
-        E[y] = imin(imax((int)(bits >> 23) - 127 - 7, -118), 120);
-      }
-      // lane group g's block of the product: its exponent is with the lanes that hold the block's columns
-      {
-        const int src = c16 + 32 * (g & 1);
-        const int lo = __shfl(E[0], src, 64);
-        if constexpr (D == 128) {
-          const int hi = __shfl(E[D / 64 - 1], src, 64);
-          const int mine = g < 2 ? lo : hi;
-#pragma unroll
-          for (int z = 0; z < PRODUCTS; ++z) qs[t][z] = mine + 127 - 4 * z;
+      for (int i = 0; i < KS; ++i) {
+        if constexpr (BF16) {
+          qt[t][0][i] = qraw[t][i];
         } else {
+          const unsigned xs[4] = {qraw[t][i].x, qraw[t][i].y, qraw[t][i].z, qraw[t][i].w};
+          unsigned hi[4], lo[4];
 #pragma unroll
-          for (int z = 0; z < PRODUCTS; ++z) qs[t][z] = lo + 127 - 4 * (2 * z + (g >> 1));
-        }
-      }
-#pragma unroll
-      for (int z = 0; z < PRODUCTS; ++z) qt[t][z] = f4_i32x8{0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {  // four columns
-        float rest[4];
-#pragma unroll
-        for (int z = 0; z < TERMS; ++z) {
-          const float scale = __uint_as_float((unsigned)(E[i / 4] + 127 - 4 * z) << 23);
-          f4_s16x2 word = {0, 0};
-          if (z == 0) {
-            if constexpr (BF16) {
-              word = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(word, __builtin_bit_cast(fp4_bf16x2, w[2 * i]), scale, false);
-              word = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(word, __builtin_bit_cast(fp4_bf16x2, w[2 * i + 1]), scale, true);
-            } else {
-              word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(word, __builtin_bit_cast(fp4_f16x2, w[2 * i]), scale, false);
-              word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(word, __builtin_bit_cast(fp4_f16x2, w[2 * i + 1]), scale, true);
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              if constexpr (BF16) {
-                rest[2 * y] = __uint_as_float(w[2 * i + y] << 16);
-                rest[2 * y + 1] = __uint_as_float(w[2 * i + y] & 0xffff0000u);
-              } else {
-                const fp4_f16x2 f = __builtin_bit_cast(fp4_f16x2, w[2 * i + y]);
-                rest[2 * y] = (float)f[0];
-                rest[2 * y + 1] = (float)f[1];
-              }
-            }
-          } else {
-            word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(word, rest[0], rest[1], scale, false);
-            word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(word, rest[2], rest[3], scale, true);
+          for (int y = 0; y < 4; ++y) {
+            const fp4_f16x2 f = __builtin_bit_cast(fp4_f16x2, xs[y]);
+            const float f0 = (float)f[0], f1 = (float)f[1];
+            hi[y] = fp4_pack_bf16(f0, f1);
+            const float h0 = __uint_as_float(hi[y] << 16), h1 = __uint_as_float(hi[y] & 0xffff0000u);
+            // (an infinity less itself is NaN: so is its row without it)
+            lo[y] = fp4_pack_bf16(f0 - h0, f1 - h1);
           }
-          const unsigned bits = __builtin_bit_cast(unsigned, word);
-          if (z + 1 < TERMS) {
-            const f4_f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(bits, scale, false), c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(bits, scale, true);
-            rest[0] -= a[0];
-            rest[1] -= a[1];
-            rest[2] -= c[0];
-            rest[3] -= c[1];
-          }
-          if constexpr (D == 128) qt[t][z][i] = (int)bits;
-          else qt[t][z / 2][4 * (z & 1) + i] = (int)bits;
+          qt[t][0][i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          qt[t][TERMS - 1][i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
-      }
-      if (__any(bad)) {  // an infinity or a NaN: the row's scores are NaN
-        asm volatile("");
-#pragma unroll
-        for (int i = 0; i < 8; ++i) qt[t][0][i] = bad ? 0x7f7f7f7f : qt[t][0][i];
       }
     }
 
@@ -430,29 +382,18 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
       f4_f32x4 s[NT][2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const f4_i32x8 a = {(int)r.k[x][0], (int)r.k[x][1], (int)r.k[x][2], (int)r.k[x][3], 0, 0, 0, 0};
+        const float sc = __uint_as_float(r.ks[x] << 23);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          s[t][x] = f4_f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NT; ++t) s[t][x] = f4_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int z = PRODUCTS - 1; z >= 0; --z)  // (small terms first)
-            s[t][x] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qt[t][z], s[t][x], 4, 0, 0, (int)r.ks[x], 0, qs[t][z]);
-        }
-      }
-      // The product does not turn a scale byte of 255 into NaN: such keys' scores are set.  (Lane (c16, .) holds scale
-      // bytes of key c16, lane (., g) the scores of keys 4 g ..)
-      if (__any(imax((int)r.ks[0], (int)r.ks[1]) == 255)) {
-        asm volatile("");  // (kept behind its branch: the compiler would rather compute it for every tile)
+        for (int i = 0; i < KS; ++i) {
+          const unsigned word = r.k[x][i];
+          const f4_bf16x8 a = __builtin_bit_cast(f4_bf16x8, make_uint4(fp4_bf16<0>(word, sc), fp4_bf16<1>(word, sc), fp4_bf16<2>(word, sc), fp4_bf16<3>(word, sc)));
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          unsigned long long nan = __ballot(r.ks[x] == 255u);
-          nan |= nan >> 32;
-          nan |= nan >> 16;
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int y = 0; y < 4; ++y)
-            if ((nan >> (4 * g + y)) & 1)
-#pragma unroll
-              for (int t = 0; t < NT; ++t) s[t][x][y] = __builtin_nanf("");
+            for (int z = TERMS - 1; z >= 0; --z)
+              s[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(f4_bf16x8, qt[t][z][i]), s[t][x], 0, 0, 0);
         }
       }
       if (TAIL && tile * kBlockN + kBlockN > n) {
@@ -558,7 +499,7 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
     if (more) {
       off = -kFp4Begin;
       do ++b;
-      while (fp4_sload(p.seq_lens + b) <= 0);  // (tiles are left, so a request follows)
+      while (fp4_len_of(p, plan, b) <= 0);  // (tiles are left, so a request follows)
       start();
     }
 
@@ -629,14 +570,14 @@ __global__ __launch_bounds__(D / 4 * PIECES < 256 ? 256 : D / 4 * PIECES) void f
   __shared__ float sm_o[ROWS][PIECES][D];
   const int tid = threadIdx.x, lane = tid & 63;
   const int b = blockIdx.y;
-  const int n = fp4_len(p, fp4_sload(p.seq_lens + b));
-  if (n <= 0) return;
+  if (fp4_sload(p.seq_lens + b) <= 0) return;
   // where the request lies among all, and the spans that hold its tiles
   const Fp4Plan plan = fp4_plan(p, lane);
+  const int n = fp4_len_of(p, plan, b);
   const int span = fp4_span(plan.total, p.spans);
   const int src = b / plan.per;
   int start = __builtin_amdgcn_readlane(plan.before, src);
-  for (int x = src * plan.per; x < b; ++x) start += fp4_cost(fp4_len(p, fp4_sload(p.seq_lens + x)));
+  for (int x = src * plan.per; x < b; ++x) start += fp4_cost(fp4_len_of(p, plan, x));
   start += kFp4Begin;  // its first tile
   const int first = start / span, pieces = (start + fp4_tiles(n) - 1) / span - first + 1;
   if (pieces <= 1) return;
@@ -710,7 +651,9 @@ static void fp4_launch(const Fp4DecodeParams& p, hipStream_t s) {
   if (R <= 8) fp4_decode_kernel<D, BF16, 1, true><<<grid, 256, 0, s>>>(p);
   else if (R <= 16) fp4_decode_kernel<D, BF16, 1, false><<<grid, 256, 0, s>>>(p);
   else fp4_decode_kernel<D, BF16, 2, false><<<grid, 256, 0, s>>>(p);
-  // pieces of a request that are joined side by side: as many as an average one can have
+  // Pieces of a row that are joined side by side, by how many an average request can have (four more of each are in
+  // flight): 16 x 4 drafted rows of up to 5 pieces 5.3 us with 2 side by side, 8.3 with 8; 8 requests of 64 pieces 5.0 with 8,
+  // 6.8 with 2, 5.2 with 32.
   const unsigned rows = (unsigned)(p.m * p.H);
   const int pieces = p.spans / p.batch;
   auto join = [&](auto pieces_) {
@@ -718,8 +661,8 @@ static void fp4_launch(const Fp4DecodeParams& p, hipStream_t s) {
     constexpr unsigned threads = D / 4 * P < 256 ? 256 : D / 4 * P, per = threads / (D / 4 * P);
     fp4_join_kernel<D, BF16, P><<<dim3((rows + per - 1) / per, (unsigned)p.batch), threads, 0, s>>>(p);
   };
-  if (pieces < 4) join(std::integral_constant<int, 2>{});
-  else if (pieces < 24) join(std::integral_constant<int, 8>{});
+  if (pieces < 8) join(std::integral_constant<int, 2>{});
+  else if (pieces <= 64) join(std::integral_constant<int, 8>{});
   else join(std::integral_constant<int, 32>{});
 }
 
@@ -756,7 +699,8 @@ extern "C" int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* a, void* st
                 (double)a->scale);
   TMX_CHECK_SUPPORTED(a->page_size >= 16 && a->page_size <= (1 << 20) && (a->page_size & (a->page_size - 1)) == 0,
                       "tmx_decode_attention_fp4: page_size %d not supported (powers of two from 16 to 2^20 are)", a->page_size);
-  TMX_CHECK_SUPPORTED(a->num_kv_heads <= 1024, "tmx_decode_attention_fp4: more than 1024 K/V heads");
+  TMX_CHECK_SUPPORTED(a->num_kv_heads <= 1024 && fp4_page_bytes(a->num_kv_heads, a->page_size, a->head_dim) <= 0x7fffffff,
+                      "tmx_decode_attention_fp4: more than 1024 K/V heads, or a page of 2^31 bytes or more");
   if (a->batch == 0) return TMX_OK;
   TMX_CHECK_ARG(a->q && a->out && a->k && a->v && a->seq_lens && a->block_table, "tmx_decode_attention_fp4: NULL tensor");
   TMX_CHECK_ARG(a->num_pages > 0 && a->num_pages <= 0x7fffffff && a->max_blocks >= 0 && a->block_table_stride >= 0,
@@ -772,7 +716,7 @@ extern "C" int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* a, void* st
                 "tmx_decode_attention_fp4: strides must not be negative, those of q multiples of 8 elements");
   // tiles of a step are counted in 32 bits
   const int64_t len_cap = (int64_t)a->max_blocks * a->page_size + a->rows_per_request;
-  TMX_CHECK_SUPPORTED(len_cap <= 0x7fffff00 && (len_cap / kBlockN + 2 + kFp4Begin) * a->batch <= 0x7fffff00,
+  TMX_CHECK_SUPPORTED(len_cap <= 0x7fffff00 && (len_cap / kBlockN + 2 + kFp4Begin) * a->batch <= 0x7fff0000,
                       "tmx_decode_attention_fp4: the block table has room for more than 2^31 tiles of 32 keys");
   int cus = 0;
   {
