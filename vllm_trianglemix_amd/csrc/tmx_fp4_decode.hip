@@ -126,9 +126,9 @@ __device__ __forceinline__ int fp4_len_of(const Fp4DecodeParams& p, const Fp4Pla
 }
 
 // Workgroups resident per CU.  Two per CU with a tile read ahead per wave have 70 KB in flight, all that the memory
-// system takes; a third only makes more pieces to change over between (64 x 8192 tokens, head size 128: 96.5 us with two,
-// 104 with three).  Head size 64 has half the bytes per tile: 65.7 us with three, 69 with two, 75 with four.
-constexpr int fp4_wgs_per_cu(int head_dim, int rows) { return head_dim == 128 || rows > 16 ? 2 : 3; }
+// system takes: a third gains nothing (64 x 8192 tokens, head size 128: 101 us with two, 100 with three; 32 ragged requests
+// 36.6 and 36.1).  Head size 64 has half the bytes per tile (64 x 8192, fp16: 64.6 us with four, 68.5 with three).
+constexpr int fp4_wgs_per_cu(int head_dim, int rows) { return head_dim == 128 || rows > 16 ? 2 : 4; }
 
 // NT column tiles of 16 rows; HALF: one tile, at most 8 rows, columns 8..15 carry the probabilities' second terms
 template <int D, bool BF16, int NT, bool HALF>

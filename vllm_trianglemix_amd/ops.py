@@ -813,11 +813,19 @@ def _fp4_caches(key_cache: torch.Tensor, value_cache: torch.Tensor) -> int:
     return 64 if width == 34 else 128
 
 
+def _module():
+    """The extension itself (its functions over lists of caches), or None when the ctypes binding serves."""
+    if _op_binding() is None:
+        return None
+    from . import torch_ops
+    return torch_ops.module
+
+
 def _call(op, *args):
-    """A registered operator's call: its refusals come as TmxError, like the library's own."""
+    """A call of the extension: its refusals come as TmxError, like the library's own."""
     try:
-        return op.default(*args)
-    except (RuntimeError, NotImplementedError) as e:
+        return op(*args)
+    except (RuntimeError, NotImplementedError, TypeError) as e:
         raise _lib.TmxError(-1, str(e)) from None
 
 
@@ -837,7 +845,7 @@ def reshape_and_cache_fp4(key: torch.Tensor, value: torch.Tensor, key_cache: tor
     _require_gpu(key_cache, "key_cache")
     C = _op_binding()
     if C is not None:
-        _call(C.trianglemix_reshape_and_cache_fp4, key, value, key_cache, value_cache, slot_mapping)
+        _call(C.trianglemix_reshape_and_cache_fp4.default, key, value, key_cache, value_cache, slot_mapping)
         return
     d = _fp4_caches(key_cache, value_cache)
     dev = key_cache.device
@@ -873,7 +881,7 @@ def gather_dequant_kv_fp4(key_cache: torch.Tensor, value_cache: torch.Tensor, bl
         k_rows, v_rows = out
         if k_rows.dtype != out_dtype:
             raise RuntimeError("output rows must be contiguous [>= total_rows, Hkv, D] of out_dtype")
-        _call(C.trianglemix_gather_dequant_kv_fp4, k_rows, v_rows, key_cache, value_cache, block_table, seq_lens, cu_seqlens_k,
+        _call(C.trianglemix_gather_dequant_kv_fp4.default, k_rows, v_rows, key_cache, value_cache, block_table, seq_lens, cu_seqlens_k,
               int(total_rows), int(max_seq_len))
         return k_rows, v_rows
     d = _fp4_caches(key_cache, value_cache)
@@ -934,7 +942,7 @@ def decode_attention_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out:
     _require_gpu(k, "k")
     C = _op_binding()
     if C is not None:
-        _call(C.trianglemix_decode_attention_fp4, out, q, k, v, block_table, seq_lens, workspace[0], workspace[1], float(scale),
+        _call(C.trianglemix_decode_attention_fp4.default, out, q, k, v, block_table, seq_lens, workspace[0], workspace[1], float(scale),
               int(rows_per_request))
         return out
     d = _fp4_caches(k, v)
@@ -1016,9 +1024,9 @@ def copy_pages(caches: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
     any cache type, usually the K and V caches of all layers.  Pairs with a number outside the pool are skipped; no page
     may be the target of two pairs, or of one and the source of another."""
     _require_gpu(pairs, "pairs")
-    C = _op_binding()
+    C = _module()
     if C is not None:
-        _call(C.trianglemix_copy_pages, caches, pairs)
+        _call(C.copy_pages, caches, pairs)
         return
     dev = pairs.device
     at, size, stride, pages = _page_list(caches, dev)
@@ -1036,7 +1044,7 @@ def free_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, num_pages: int
     _require_gpu(block_table, "block_table")
     C = _op_binding()
     if C is not None:
-        return _call(C.trianglemix_free_pages, block_table, seq_lens, int(num_pages), int(page_size))
+        return _call(C.trianglemix_free_pages.default, block_table, seq_lens, int(num_pages), int(page_size))
     dev = _page_table(block_table, seq_lens)
     if num_pages < 0:
         raise RuntimeError("num_pages must not be negative")
@@ -1058,9 +1066,9 @@ def fork_pages(caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq_le
     that is no row gives a row of -1.  The fresh pages (:func:`free_pages`) are distinct and not in use; one whose parent
     ends on a page boundary stays free."""
     _require_gpu(block_table, "block_table")
-    C = _op_binding()
+    C = _module()
     if C is not None:
-        return _call(C.trianglemix_fork_pages, caches, block_table, seq_lens, parents, fresh, int(page_size))
+        return _call(C.fork_pages, caches, block_table, seq_lens, parents, fresh, int(page_size))
     dev = _page_table(block_table, seq_lens)
     at, size, stride, pages = _page_list(caches, dev)
     _on(dev, (parents, "parents"), (fresh, "fresh"))
@@ -1081,9 +1089,9 @@ def compact_pages(caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq
     afterwards (a new int32 ``[rows, max_blocks]``, -1 behind a row's entries) and U (int32 ``[1]``).  Pages shared by
     several rows move once.  Nothing is read back to the host."""
     _require_gpu(block_table, "block_table")
-    C = _op_binding()
+    C = _module()
     if C is not None:
-        return _call(C.trianglemix_compact_pages, caches, block_table, seq_lens, int(page_size))
+        return _call(C.compact_pages, caches, block_table, seq_lens, int(page_size))
     dev = _page_table(block_table, seq_lens)
     if not len(caches):
         raise RuntimeError("compact_pages needs the caches (their first dimension is the pool)")

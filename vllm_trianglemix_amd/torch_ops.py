@@ -13,16 +13,17 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 BINDING_PATH = os.path.join(_HERE, "_trianglemix_C.so")
 _loaded = False
+module = None  # the extension itself: the operators over lists of caches as plain functions
 
 
 def load():
     """Registers the ops (once) and returns ``torch.ops._trianglemix_C``."""
-    global _loaded
+    global _loaded, module
     if not _loaded:
         if not os.path.exists(BINDING_PATH):
             raise ImportError(f"{BINDING_PATH} is missing: build it with `make -C {os.path.join(_HERE, 'csrc')}`")
         # a plain import: the shared object is a Python extension module whose load registers the ops
         # (PyInit__trianglemix_C, the reference's REGISTER_EXTENSION, csrc/core/registration.h:13-27)
-        importlib.import_module(__package__ + "._trianglemix_C")
+        module = importlib.import_module(__package__ + "._trianglemix_C")
         _loaded = True
     return torch.ops._trianglemix_C
