@@ -442,6 +442,30 @@ def test_gather_returns_the_values_the_cache_stands_for(dtype, dim, heads, page)
 
 
 @gpu
+def test_caches_past_4_gib():
+    """Pages half a GiB apart: every offset of the last ones needs more than 32 bits."""
+    b = Batch(18, [100, 61], 8, 2, 128, 16, page_gap=(1 << 29) - 16 * 2 * 68)
+    assert b.caches[0].stride(0) == 1 << 29 and int(b.table.max()) * (1 << 29) > 1 << 32
+    b.check(torch.bfloat16)
+    cu = torch.tensor([0, 100, 161], dtype=torch.int32, device=DEV)
+    k, v = ops.gather_dequant_kv_fp4(*b.caches, b.bt, b.sl, cu, 161, 100, torch.bfloat16)
+    for x, got in enumerate((k, v)):
+        assert np.array_equal(got.double().cpu().numpy(), np.concatenate([b.keys(0)[x], b.keys(1)[x]]))
+    rows = torch.randn(161, 2, 128, device=DEV).bfloat16()
+    pos = [np.arange(n) for n in (100, 61)]
+    slots = np.concatenate([b.table[i, p // 16].astype(np.int64) * 16 + p % 16 for i, p in enumerate(pos)])
+    ops.reshape_and_cache_fp4(rows, -rows, *b.caches, torch.from_numpy(slots).to(DEV))
+    k, v = ops.gather_dequant_kv_fp4(*b.caches, b.bt, b.sl, cu, 161, 100, torch.bfloat16)
+    want = ref.values(*ref.quantise(rows.double().cpu().numpy()))
+    assert np.array_equal(k.double().cpu().numpy(), want) and torch.equal(v, -k)
+    # and the pages as pages
+    last = int(b.table[:, :4].max())
+    other = int((set(range(b.caches[0].shape[0])) - set(b.table.ravel().tolist())).pop())
+    ops.copy_pages(b.caches, torch.tensor([[last, other]], device=DEV))
+    assert torch.equal(b.caches[0][last], b.caches[0][other]) and torch.equal(b.caches[1][last], b.caches[1][other])
+
+
+@gpu
 def test_fp16_rows_saturate():
     x = torch.full((1, 1, 64), 65504.0, dtype=torch.float16, device=DEV)
     x[0, 0, 1] = -65504.0

@@ -208,8 +208,9 @@ def test_more_caches_than_one_launch_takes():
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(3, 32), (16, 8, 68)])
 @pytest.mark.parametrize("rows, cols, page, children", [(1, 1, 16, 1), (3, 5, 16, 7), (8, 300, 16, 40), (4, 9, 1, 5), (5, 6, 64, 3)])
-def test_fork_pages(rows, cols, page, children):
+def test_fork_pages(rows, cols, page, children, shape):
     rng = np.random.default_rng(rows + cols)
     pages = rows * cols + children + 3
     table, lens = random_tables(rng, rows, cols, pages - children, page, share=0.0)
@@ -222,7 +223,7 @@ def test_fork_pages(rows, cols, page, children):
     if children > 3:
         parents[1], parents[2] = -1, rows  # no such row
     fresh = np.arange(pages - children, pages).astype(np.int32)
-    start = [torch.randint(0, 256, (pages, 3, 32), dtype=torch.uint8) for _ in range(4)]
+    start = [torch.randint(0, 256, (pages, *shape), dtype=torch.uint8) for _ in range(4)]
     got = [x.to(DEV) for x in start]
     child = ops.fork_pages(got, t32(table), t32(lens), t32(parents), t32(fresh), page)
     want, copies = plain_fork(table, lens, parents, fresh, page)
@@ -268,6 +269,48 @@ def test_captured_page_operators_replay_on_other_tables():
             if move:
                 x[list(move.values())] = x[list(move.keys())]
             assert torch.equal(y.cpu(), x)
+
+
+@gpu
+def test_empty_tables():
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    c = [torch.arange(5 * 32, dtype=torch.uint8, device=DEV).view(5, 32)]
+    for bt in (torch.zeros(0, 4, dtype=torch.int32, device=DEV), torch.zeros(0, 0, dtype=torch.int32, device=DEV)):
+        free, n = ops.free_pages(bt, none, 5, 16)
+        assert free.tolist() == [0, 1, 2, 3, 4] and int(n) == 5
+        table, used = ops.compact_pages(c, bt, none, 16)
+        assert table.shape == bt.shape and int(used) == 0
+        assert ops.fork_pages(c, bt, none, none, none, 16).shape == bt.shape
+    free, n = ops.free_pages(torch.zeros(2, 4, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV), 0, 16)
+    assert free.numel() == 0 and int(n) == 0
+    assert torch.equal(c[0].flatten().cpu(), torch.arange(5 * 32, dtype=torch.uint8))
+
+
+@gpu
+def test_the_registered_operators_do_the_same():
+    from vllm_trianglemix_amd import torch_ops
+    C = torch_ops.load()
+    rng = np.random.default_rng(6)
+    table, lens = random_tables(rng, 6, 9, 60, 16)
+    start = torch.randint(0, 256, (3, 64, 48), dtype=torch.uint8, device=DEV)
+    bt, sl = t32(table), t32(lens)
+    one, two = list(start.clone()), list(start.clone())
+    free, n = ops.free_pages(bt, sl, 64, 16)
+    free2, n2 = C.trianglemix_free_pages(bt, sl, 64, 16)
+    assert torch.equal(free, free2) and int(n) == int(n2)
+    parents = t32([0, 3])
+    assert torch.equal(ops.fork_pages(one, bt, sl, parents, free[:2], 16), C.trianglemix_fork_pages(two, bt, sl, parents, free[:2], 16))
+    a, b = ops.compact_pages(one, bt, sl, 16), C.trianglemix_compact_pages(two, bt, sl, 16)
+    assert torch.equal(a[0], b[0]) and int(a[1]) == int(b[1])
+    pairs = torch.tensor([[1, 60], [2, 61]], device=DEV)
+    ops.copy_pages(one, pairs)
+    C.trianglemix_copy_pages(two, pairs)
+    assert torch.equal(torch.stack(one), torch.stack(two))
+    with pytest.raises(RuntimeError):
+        C.trianglemix_copy_pages(two, pairs.float())
+    for bad in ((one, None), (pairs, pairs), ([pairs, 3], pairs), (one,)):
+        with pytest.raises(RuntimeError):
+            torch_ops.module.copy_pages(*bad)
 
 
 @gpu

@@ -12,10 +12,10 @@
 //   queries are split into two bf16 terms (exact: 11 bits in 8 + 8).  (The scaled product that takes 4-bit operands as
 //   they are would save these conversions, but it sums 8 neighbouring products with some 14 bits below the largest of
 //   them: a query column 2^7 below its neighbours would not count.)
-//   Output O^T = V^T P^T (the same product): lane (m, g) needs columns [m D/16, (m + 1)
-//   D/16) of the 8 keys whose scores it holds, 4 g .. 4 g + 3 and 16 + 4 g .. + 3.  The cache keeps V in that order
-//   (tmx_fp4.h), so V comes straight from memory, becomes bf16 by 32
-//   conversions and is paired by 32 byte permutes; the probabilities never leave their lane.  No LDS in the loop.
+//   Output O^T = V^T P^T (the same product): lane (m, g) needs columns [m D/16, (m + 1) D/16) of the 8 keys whose scores
+//   it holds, 4 g .. 4 g + 3 and 16 + 4 g .. + 3.  The cache keeps V in that order (tmx_fp4.h), so V comes straight from
+//   memory, becomes bf16 by 32 conversions and is paired by 32 byte permutes; the probabilities never leave their lane.
+//   No LDS in the loop.
 //   Probabilities are held as two bf16 terms (16 significant bits; one term alone would cost as much accuracy as the
 //   rounding of the output).  Up to 8 rows, columns 8..15 repeat the rows and carry the second term: no extra product.
 //   Their sum is one more product, with ones.
@@ -165,11 +165,10 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
     const int src = __builtin_ctzll(own);  // (one lane holds it: begin < total)
     b = src * plan.per;
     int at = __builtin_amdgcn_readlane(plan.before, src);
-    for (;;) {
+    for (; b < p.batch - 1; ++b) {
       const int cj = fp4_cost(fp4_len_of(p, plan, b));
       if (begin < at + cj) break;
       at += cj;
-      ++b;
     }
     off = begin - at - kFp4Begin;  // (negative: the request begins in this span)
     left = imin(plan.total - begin, span);
@@ -495,11 +494,15 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
 
     // ---- the piece is done; the next one's loads go out before it is written ----
     const int b_done = b, n_done = n;
-    const bool whole_done = whole, more = left > kFp4Begin;
+    const bool whole_done = whole;
+    bool more = left > kFp4Begin;
+    if (more) {
+      do ++b;
+      while (b < p.batch && fp4_len_of(p, plan, b) <= 0);
+      more = b < p.batch;
+    }
     if (more) {
       off = -kFp4Begin;
-      do ++b;
-      while (fp4_len_of(p, plan, b) <= 0);  // (tiles are left, so a request follows)
       start();
     }
 

@@ -7,6 +7,8 @@
 // ceil(lens[r] / page_size) entries -- so there is no count to keep in step: a sequence is freed by setting its length to
 // 0.  "In use" is one bit per page; with a running count per 32-bit word every page knows its rank among the used
 // (or free) ones, which is its place in every list here: no list depends on the order in which workgroups run.
+#include <type_traits>
+
 #include "tmx_common.h"
 
 namespace tmx {
@@ -92,8 +94,8 @@ __device__ __forceinline__ int pg_moved(const unsigned* bits, const int* count, 
 
 enum { PG_FREE = 0, PG_COMPACT = 1 };
 
-// ---- one workgroup does it all, bits and counts in LDS: tables of up to kPageSmall entries.  One launch instead of four
-// or five (two to three microseconds apiece on an idle queue); see the launch for both sides measured. ----
+// ---- one workgroup does it all, bits and counts in LDS: tables of up to kPageSmall entries (both sides measured where it
+// is launched) ----
 template <int WHAT>
 __global__ __launch_bounds__(1024) void pg_small_kernel(const PageTable t, int32_t* __restrict__ list, int32_t* __restrict__ total,
                                                          int32_t* __restrict__ new_table) {
@@ -185,46 +187,56 @@ __global__ __launch_bounds__(256) void pg_table_kernel(const PageTable t, const 
 // before the next cache's, so that the pages in flight lie close together (595 us pair by pair); loads and stores past the
 // caches (555 us with neither, 568 with cached stores); a grid of 2048 workgroups that take further chunks in turn (8 per
 // CU: 524 to 530 us from 1536 to 4096). ----
-// One chunk of a page, `units` 16-byte units, by the workgroup: a thread's four loads are under way before its first
-// store (two at a time: 549 us).
-constexpr int kChunkUnits = 4 * 256;
+// A chunk of a page, `units` 16-byte units, is copied by LANES threads: a whole workgroup, or one wave where a page is so
+// small that most of a workgroup would idle (pages up to 4 KB: 8928 copies of 1088 bytes 5.6 us by waves, 9.7 by workgroups;
+// 72000 of 8704 bytes 269 and 264).  A thread's four loads are under way before its first store (two at a time: 549 us for
+// the case above).
+template <int LANES>
 __device__ __forceinline__ void pg_copy_chunk(const char* src, char* dst, int units) {
   typedef __attribute__((ext_vector_type(4))) unsigned u4;
+  const int lane = (int)threadIdx.x & (LANES - 1);
   u4 x[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int u = i * 256 + (int)threadIdx.x;
+    const int u = i * LANES + lane;
     if (u < units) x[i] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(src) + u);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int u = i * 256 + (int)threadIdx.x;
+    const int u = i * LANES + lane;
     if (u < units) __builtin_nontemporal_store(x[i], reinterpret_cast<u4*>(dst) + u);
   }
+}
+// this copier's number among the launch's, and how many there are
+template <int LANES>
+__device__ __forceinline__ unsigned pg_copier() {
+  return __builtin_amdgcn_readfirstlane(blockIdx.x * (256u / LANES) + threadIdx.x / LANES);
 }
 
 struct PageShape {
   int64_t stride;    // bytes from page to page
   int units;         // 16-byte units of a page
-  int chunk, chunks; // units per chunk, chunks per page
+  int lanes;         // threads that copy a chunk: 64 or 256
+  int chunk, chunks; // units per chunk (at most 4 x lanes), chunks per page
   int num_pages, num_caches;
 };
 
-template <typename T>
+template <typename T, int LANES>
 __global__ __launch_bounds__(256) void pg_copy_kernel(const PageCaches caches, const PageShape s, const T* __restrict__ pairs, int cap,
                                                       const int32_t* __restrict__ count) {
-  const int n = count ? imin(cap, *count) : cap;
+  const int n = count ? imax(0, imin(cap, *count)) : cap;
   const unsigned items = (unsigned)n * s.num_caches * s.chunks;  // (below 2^31: checked before the launch)
-  for (unsigned i = blockIdx.x; i < items; i += gridDim.x) {
+  for (unsigned i = pg_copier<LANES>(); i < items; i += gridDim.x * (256u / LANES)) {
     const unsigned pc = i / (unsigned)s.chunks, cache = pc / (unsigned)n;
     const int ch = (int)(i - pc * s.chunks), pair = (int)(pc - cache * n);
     const int64_t a = pairs[2ll * pair], b = pairs[2ll * pair + 1];
     if (a < 0 || b < 0 || a >= s.num_pages || b >= s.num_pages || a == b) continue;
     const int u0 = ch * s.chunk;
-    pg_copy_chunk(caches.at[cache] + a * s.stride + 16ll * u0, caches.at[cache] + b * s.stride + 16ll * u0, imin(s.chunk, s.units - u0));
+    pg_copy_chunk<LANES>(caches.at[cache] + a * s.stride + 16ll * u0, caches.at[cache] + b * s.stride + 16ll * u0, imin(s.chunk, s.units - u0));
   }
 }
 
+template <int LANES>
 __global__ __launch_bounds__(256) void pg_fork_kernel(const PageCaches caches, const PageShape s, const PageTable t,
                                                       const int32_t* __restrict__ parents, const int32_t* __restrict__ fresh, int children,
                                                       int32_t* __restrict__ child_table) {
@@ -246,7 +258,7 @@ __global__ __launch_bounds__(256) void pg_fork_kernel(const PageCaches caches, c
     }
   }
   const unsigned items = (unsigned)children * s.num_caches * s.chunks;
-  for (unsigned i = blockIdx.x; i < items; i += gridDim.x) {
+  for (unsigned i = pg_copier<LANES>(); i < items; i += gridDim.x * (256u / LANES)) {
     const unsigned pc = i / (unsigned)s.chunks, cache = pc / (unsigned)children;
     const int ch = (int)(i - pc * s.chunks), child = (int)(pc - cache * children);
     const int r = parents[child];
@@ -256,11 +268,11 @@ __global__ __launch_bounds__(256) void pg_fork_kernel(const PageCaches caches, c
     const int a = t.table[r * t.stride + full], b = fresh[child];
     if (a < 0 || b < 0 || a >= s.num_pages || b >= s.num_pages || a == b) continue;
     const int u0 = ch * s.chunk;
-    pg_copy_chunk(caches.at[cache] + a * s.stride + 16ll * u0, caches.at[cache] + b * s.stride + 16ll * u0, imin(s.chunk, s.units - u0));
+    pg_copy_chunk<LANES>(caches.at[cache] + a * s.stride + 16ll * u0, caches.at[cache] + b * s.stride + 16ll * u0, imin(s.chunk, s.units - u0));
   }
 }
 
-constexpr int64_t kPageSmall = 65536;      // table entries up to which one workgroup makes the plan
+constexpr int64_t kPageSmall = 16384;      // table entries up to which one workgroup makes the plan
 constexpr int kPageSmallPages = 1 << 17;   // pages whose bits and counts it holds in LDS (32 KB)
 
 static int pg_check_table(const char* fn, const int32_t* table, int64_t stride, int rows, int cols, const int32_t* lens, int page_size,
@@ -281,13 +293,14 @@ static int pg_shape(const char* fn, void* const* caches, int num_caches, int64_t
                       (long long)page_bytes, (long long)stride_page);
   TMX_CHECK_ARG(stride_page >= page_bytes, "%s: pages overlap (stride %lld, %lld bytes)", fn, (long long)stride_page, (long long)page_bytes);
   TMX_CHECK_ARG(num_caches == 0 || caches != nullptr, "%s: NULL pointer", fn);
-  const int64_t chunks = (page_bytes / 16 + kChunkUnits - 1) / kChunkUnits;
+  s->units = (int)(page_bytes / 16);
+  s->lanes = page_bytes <= 4096 ? 64 : 256;
+  const int64_t chunks = (s->units + 4 * s->lanes - 1) / (4 * s->lanes);
   TMX_CHECK_SUPPORTED(copies * imin(num_caches, kPagesPerLaunch) * chunks <= 0x7fffffff, "%s: too many copies for one call", fn);
   for (int i = 0; i < num_caches; ++i)
     TMX_CHECK_ARG(caches[i] != nullptr && (uintptr_t)caches[i] % 16 == 0, "%s: cache %d is NULL or not 16-byte aligned", fn, i);
   s->stride = stride_page;
-  s->units = (int)(page_bytes / 16);
-  s->chunks = (s->units + kChunkUnits - 1) / kChunkUnits;
+  s->chunks = (int)chunks;
   s->chunk = (s->units + s->chunks - 1) / s->chunks;
   s->num_pages = (int)num_pages;
   s->num_caches = num_caches;
@@ -295,7 +308,10 @@ static int pg_shape(const char* fn, void* const* caches, int num_caches, int64_t
 }
 
 // workgroups of a copy: enough to fill the chip eight deep, each takes further chunks in turn
-static unsigned pg_grid(int64_t items) { return (unsigned)(items < 2048 ? (items < 1 ? 1 : items) : 2048); }
+static unsigned pg_grid(int64_t items, int lanes) {
+  const int64_t n = (items * lanes + 255) / 256;
+  return (unsigned)(n < 1 ? 1 : (n < 2048 ? n : 2048));
+}
 
 // words of bits (and of counts), one past the last among them
 static int64_t pg_words(int64_t num_pages) { return (num_pages + 31) / 32 + 1; }
@@ -304,8 +320,8 @@ static bool pg_small(int64_t entries, int64_t num_pages) { return entries <= kPa
 template <int WHAT>
 static int pg_plan(const char* fn, const PageTable& t, int32_t* list, int32_t* total, int32_t* new_table, int32_t* work, int64_t work_ints,
                    hipStream_t s) {
-  // One workgroup reads the table at some 60 GB/s, a launch over the chip at memory speed; the single launch wins until the
-  // table's entries take longer than the launches saved.
+  // One launch against four or five: the search for free pages takes 3.0 against 8.1 us for 8 x 64 entries, 5.6 against 11.4
+  // for 64 x 128, 13.0 against 14.5 for 64 x 512 and 23.8 against 16.8 for 128 x 512; with the new table 13, 18 / 32, 26.
   if (pg_small((int64_t)t.rows * t.cols, t.num_pages)) {
     const size_t lds = 8 * (size_t)pg_words(t.num_pages);
     pg_small_kernel<WHAT><<<1, 1024, lds, s>>>(t, list, total, new_table);
@@ -374,9 +390,14 @@ extern "C" int tmx_copy_pages(void* const* caches, int32_t num_caches, int64_t p
     s.num_caches = imin(kPagesPerLaunch, num_caches - c0);
     for (int i = 0; i < s.num_caches; ++i) p.at[i] = (char*)caches[c0 + i];
     for (int i = s.num_caches; i < kPagesPerLaunch; ++i) p.at[i] = nullptr;
-    const unsigned grid = pg_grid((int64_t)num_pairs * s.num_caches * s.chunks);
-    if (pair_bits == 64) pg_copy_kernel<int64_t><<<grid, 256, 0, (hipStream_t)stream>>>(p, s, (const int64_t*)pairs, num_pairs, count);
-    else pg_copy_kernel<int32_t><<<grid, 256, 0, (hipStream_t)stream>>>(p, s, (const int32_t*)pairs, num_pairs, count);
+    const unsigned grid = pg_grid((int64_t)num_pairs * s.num_caches * s.chunks, s.lanes);
+    auto launch = [&](auto lanes) {
+      constexpr int L = decltype(lanes)::value;
+      if (pair_bits == 64) pg_copy_kernel<int64_t, L><<<grid, 256, 0, (hipStream_t)stream>>>(p, s, (const int64_t*)pairs, num_pairs, count);
+      else pg_copy_kernel<int32_t, L><<<grid, 256, 0, (hipStream_t)stream>>>(p, s, (const int32_t*)pairs, num_pairs, count);
+    };
+    if (s.lanes == 64) launch(std::integral_constant<int, 64>{});
+    else launch(std::integral_constant<int, 256>{});
     TMX_CHECK_HIP(hipGetLastError());
   }
   return TMX_OK;
@@ -403,7 +424,8 @@ extern "C" int tmx_fork_pages(void* const* caches, int32_t num_caches, int64_t p
     for (int i = 0; i < s.num_caches; ++i) p.at[i] = (char*)caches[c0 + i];
     for (int i = s.num_caches; i < kPagesPerLaunch; ++i) p.at[i] = nullptr;
     const int64_t items = (int64_t)children * (s.num_caches > 0 ? s.num_caches : 1) * s.chunks;
-    pg_fork_kernel<<<pg_grid(items), 256, 0, (hipStream_t)stream>>>(p, s, t, parents, fresh, children, c0 == 0 ? child_table : nullptr);
+    auto* kernel = s.lanes == 64 ? pg_fork_kernel<64> : pg_fork_kernel<256>;
+    kernel<<<pg_grid(items, s.lanes), 256, 0, (hipStream_t)stream>>>(p, s, t, parents, fresh, children, c0 == 0 ? child_table : nullptr);
     TMX_CHECK_HIP(hipGetLastError());
   }
   return TMX_OK;
