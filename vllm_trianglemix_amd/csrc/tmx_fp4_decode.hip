@@ -582,10 +582,10 @@ __global__ __launch_bounds__(D / 4 * PIECES < 256 ? 256 : D / 4 * PIECES) void f
   __shared__ float sm_o[ROWS][PIECES][D];
   const int tid = threadIdx.x, lane = tid & 63;
   const int b = blockIdx.y;
-  if (fp4_sload(p.seq_lens + b) <= 0) return;
   // where the request lies among all, and the spans that hold its tiles
   const Fp4Plan plan = fp4_plan(p, lane);
   const int n = fp4_len_of(p, plan, b);
+  if (n <= 0) return;
   const int span = fp4_span(plan.total, p.spans);
   const int src = b / plan.per;
   int start = __builtin_amdgcn_readlane(plan.before, src);
@@ -664,7 +664,7 @@ static void fp4_launch(const Fp4DecodeParams& p, hipStream_t s) {
   else if (R <= 16) fp4_decode_kernel<D, BF16, 1, false><<<grid, 256, 0, s>>>(p);
   else fp4_decode_kernel<D, BF16, 2, false><<<grid, 256, 0, s>>>(p);
   // Pieces of a row that are joined side by side, by how many an average request can have (four more of each are in
-  // flight): 16 x 4 drafted rows of up to 5 pieces 5.3 us with 2 side by side, 8.3 with 8; 8 requests of 64 pieces 5.0 with 8,
+  // flight): 16 x 4 drafted rows of up to 5 pieces 4.9 us with 2 side by side, 8.3 with 8; 8 requests of 64 pieces 4.5 with 8,
   // 6.8 with 2, 5.2 with 32.
   const unsigned rows = (unsigned)(p.m * p.H);
   const int pieces = p.spans / p.batch;
