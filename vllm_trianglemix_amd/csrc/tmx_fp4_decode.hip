@@ -126,9 +126,9 @@ __device__ __forceinline__ int fp4_len_of(const Fp4DecodeParams& p, const Fp4Pla
 }
 
 // Workgroups resident per CU.  Two per CU with a tile read ahead per wave have 70 KB in flight, all that the memory
-// system takes: a third gains little where spans are long and loses where they are short (whole calls on inputs that no cache
-// holds, head size 128: 64 x 8192 tokens 99.7 us with two, 98.6 with three; 4 x 16384 22.0 and 23.3; 8 x 65536 of one K/V head
-// 23.9 and 24.7).  Head size 64 has half the bytes per tile (64 x 8192, fp16: 64.4 us with four, 65.2 with three, 71.7 with two).
+// system takes (whole calls on inputs that no cache holds, head size 128: 64 x 8192 tokens 92.2 us with two, 99.1 with three, 95.4
+// with two that read two tiles ahead; 4 x 16384 21.0 and 22.9 with three; 32 ragged requests 33.2 and 35.2).  Head size 64 has
+// half the bytes per tile (64 x 8192, fp16: 64.4 us with four, 65.9 with two).
 constexpr int fp4_wgs_per_cu(int head_dim, int rows) { return head_dim == 128 || rows > 16 ? 2 : 4; }
 
 // NT column tiles of 16 rows; HALF: one tile, at most 8 rows, columns 8..15 carry the probabilities' second terms
@@ -148,14 +148,14 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
   const int c16 = lane & 15, g = lane >> 4;
   // Workgroups go round the 8 XCDs: this order gives an XCD a run of spans with all their heads, so that the heads of a
   // page -- and the cache lines in which two heads' scale bytes meet -- are read through one L2 at about the same time
-  // (64 x 8192 tokens, 32 / 8 heads: 99.7 us against 100.4 with the heads spread over the XCDs; head size 64 65.9 against 67.2).
+  // (64 x 8192 tokens, 32 / 8 heads: 92.6 us against 95.2 with the heads spread over the XCDs; head size 64 64.0 against 65.9).
   const int lin = ((int)blockIdx.x & 7) * ((int)gridDim.x >> 3) + ((int)blockIdx.x >> 3);
   const int w = lin / p.units, unit = lin - w * p.units;
   const int h = unit / p.row_groups, row0 = 32 * (unit - h * p.row_groups);
   if (w >= p.spans) return;
-  // A SIMD issues for its oldest wave first.  Of two workgroups on a CU the one launched first finished its equal span at 75 us,
-  // the other at 89 us, alone with its loads at the end.  The younger half of the grid takes precedence on every other tile:
-  // both finish at 83 us (64 x 8192 tokens: the whole call 100.5 -> 97.0 us; 32 x 4096 with 32 K/V heads 100 -> 95).
+  // A SIMD issues for its oldest wave first: of two workgroups on a CU the one launched first finished its equal span at 75 us,
+  // the other at 89 us, alone with its loads at the end.  The younger half of the grid takes precedence on every other tile, and
+  // both finish together (64 x 8192 tokens: the whole call 96.7 -> 92.2 us, 32 ragged requests 34.0 -> 33.2).
   const bool younger = blockIdx.x >= gridDim.x / 2;
 
   // the request at which this workgroup's span begins, and where in it
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_ke
       const int scales = scales_from_codes + at - at * (D / 2);
       const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.k) + base, 0, size, 0x00020000);
       const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.v) + base, 0, size, 0x00020000);
-      constexpr int kStream = 2;  // codes are read once: non-temporal (64 x 8192: 99.7 against 105.7 us; 32 ragged requests 34.7 and 38.5)
+      constexpr int kStream = 2;  // codes are read once: non-temporal (64 x 8192: 92.2 against 106.0 us; 32 ragged requests 33.2 and 38.3)
       if constexpr (D == 128) {
         const fp4_u32x4 z = __builtin_bit_cast(fp4_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_lane, 0, kStream));
 #pragma unroll
