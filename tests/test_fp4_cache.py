@@ -422,6 +422,38 @@ def test_pages_that_do_not_exist_count_as_nan():
 
 
 @gpu
+@pytest.mark.parametrize("page", [16, 64])
+def test_entries_past_a_sequence_are_not_used(page):
+    """The table is looked up ahead of the tiles, past a sequence's last one too: what stands there does not matter, and a
+    table just wide enough does as well."""
+    lens = [32, 512, 1, 480, 33, 96]
+    b = Batch(23, lens, 8, 2, 128, page)
+    _, want = b.run(torch.bfloat16)
+    width = max(-(-n // page) for n in lens)
+    wide = torch.full((len(lens), width + 40), 2 ** 31 - 1, dtype=torch.int32, device=DEV)
+    for r, n in enumerate(lens):
+        wide[r, :-(-n // page)] = b.bt[r, :-(-n // page)]
+    for table in (wide, wide[:, :width], wide[:, :width].contiguous()):
+        b.bt = table
+        assert torch.equal(b.run(torch.bfloat16)[1], want)
+
+
+@gpu
+def test_a_table_without_columns():
+    """Through the C interface (an empty tensor has no address): sequences with keys and no pages are NaN."""
+    b = Batch(29, [3, 0, 40], 8, 2, 128, 16)
+    q = torch.from_numpy(b.q).to(torch.bfloat16).to(DEV)
+    out = torch.zeros_like(q)
+    ws = ops.decode_fp4_workspace(3, 1, 8, 2, 128, DEV)
+    a = _args(batch=3, q=q.data_ptr(), out=out.data_ptr(), k=b.caches[0].data_ptr(), v=b.caches[1].data_ptr(), max_blocks=0,
+              block_table=b.bt.data_ptr(), seq_lens=b.sl.data_ptr(), partial_o=ws[0].data_ptr(), partial_ml=ws[1].data_ptr(),
+              workspace_rows=ws[1].numel() // 2, num_pages=b.caches[0].shape[0], kv_stride_page=b.caches[0].stride(0))
+    assert _lib.load().tmx_decode_attention_fp4(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == _lib.TMX_OK
+    torch.cuda.synchronize()
+    assert torch.isnan(out[0]).all() and torch.isnan(out[2]).all() and (out[1] == 0).all()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("dim, heads, page", [(128, 2, 16), (64, 3, 32), (128, 8, 64), (64, 1, 16)])
 def test_gather_returns_the_values_the_cache_stands_for(dtype, dim, heads, page):
