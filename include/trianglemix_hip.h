@@ -523,7 +523,7 @@ int tmx_gather_dequant_kv_fp8(const void* key_cache, const void* value_cache, in
  * already).  m = 1 is a decode step, m > 1 checks drafted tokens; m * num_heads / num_kv_heads <= 64.  seq_lens[b] <= 0
  * marks padding, its out rows are left alone, as are rows at negative positions.  As in tmx_decode_attention the launch
  * depends on the batch size alone (it replays under a graph) and the work area -- partial_o [rows][head_dim], partial_ml
- * [rows][2], rows = tmx_decode_fp4_workspace_rows(...) -- belongs to one call at a time.
+ * [rows][2], rows = tmx_decode_fp4_workspace_rows(...), whatever they hold -- belongs to one call at a time.
  * ---------------------------------------------------------------------- */
 int tmx_reshape_and_cache_fp4(const void* key, const void* value, int64_t key_stride_t, int64_t key_stride_h,
                               int64_t value_stride_t, int64_t value_stride_h, void* key_cache, void* value_cache,

@@ -298,6 +298,28 @@ def test_many_requests(batch):
 
 
 @gpu
+def test_more_requests_than_workgroups():
+    """Several requests to a workgroup and to a lane of the plan, some that lie in two spans."""
+    rng = np.random.default_rng(5)
+    lens = [int(n) for n in rng.integers(0, 40, 1100)]
+    lens[700] = 900
+    Batch(1100, lens, 2, 1, 64, 16).check(torch.bfloat16)
+
+
+@gpu
+def test_one_work_area_serves_steps_of_other_sizes():
+    """What an earlier call left in the work area -- partial results, where its pieces lay -- does not reach a later one."""
+    steps = [Batch(31, [900, 1, 64, 0, 2000], 8, 2, 128, 16), Batch(32, [33], 8, 2, 128, 16), Batch(33, [5, 700, 300], 8, 2, 128, 16, m=2),
+             Batch(34, [0, 1500, 0, 40, 8], 8, 2, 128, 16)]
+    ws = max((ops.decode_fp4_workspace(len(b.lens), b.m, 8, 2, 128, DEV) for b in steps), key=lambda w: w[0].numel())
+    for b in steps * 3:
+        q, want = b.run(torch.bfloat16)
+        out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=DEV)
+        ops.decode_attention_fp4(q.to(DEV), *b.caches, out, b.bt, b.sl, b.scale, ws, rows_per_request=b.m)
+        assert torch.equal(out, want)
+
+
+@gpu
 def test_few_long_sequences_split_over_the_chip():
     Batch(5, [20011], 8, 1, 128, 16).check(torch.bfloat16, torch.float32)
     Batch(6, [9000, 1, 12345], 4, 1, 128, 64, m=2).check(torch.float16, torch.float32)
