@@ -814,7 +814,7 @@ def _fp4_caches(key_cache: torch.Tensor, value_cache: torch.Tensor) -> int:
 
 
 def _module():
-    """The extension itself (its functions over lists of caches), or None when the ctypes binding serves."""
+    """The extension itself (the page operators as plain functions), or None when the ctypes binding serves."""
     if _op_binding() is None:
         return None
     from . import torch_ops
@@ -1042,9 +1042,9 @@ def free_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, num_pages: int
     behind the last, and ``[1]``.  Row ``r`` of ``block_table`` uses its first ``ceil(seq_lens[r] / page_size)`` entries; a
     sequence is freed by a length of 0.  Nothing is read back to the host."""
     _require_gpu(block_table, "block_table")
-    C = _op_binding()
+    C = _module()
     if C is not None:
-        return _call(C.trianglemix_free_pages.default, block_table, seq_lens, int(num_pages), int(page_size))
+        return _call(C.free_pages, block_table, seq_lens, int(num_pages), int(page_size))
     dev = _page_table(block_table, seq_lens)
     if num_pages < 0:
         raise RuntimeError("num_pages must not be negative")

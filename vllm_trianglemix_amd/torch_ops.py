@@ -13,7 +13,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 BINDING_PATH = os.path.join(_HERE, "_trianglemix_C.so")
 _loaded = False
-module = None  # the extension itself: the operators over lists of caches as plain functions
+module = None  # the extension itself: the page operators as plain functions
 
 
 def load():
