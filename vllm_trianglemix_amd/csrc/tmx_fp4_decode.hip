@@ -678,8 +678,8 @@ static void fp4_launch(const Fp4DecodeParams& p, hipStream_t s) {
   else if (R <= 16) fp4_decode_kernel<D, BF16, 1, false><<<grid, 256, 0, s>>>(p);
   else fp4_decode_kernel<D, BF16, 2, false><<<grid, 256, 0, s>>>(p);
   // Pieces of a row that are joined side by side, by how many an average request can have (four more of each are in
-  // flight): 16 x 4 drafted rows of up to 5 pieces 4.9 us with 2 side by side, 8.3 with 8; 8 requests of 64 pieces 4.5 with 8,
-  // 6.8 with 2, 5.2 with 32.
+  // flight), with 2 / 8 / 32 of them: 16 x 4 drafted rows of up to 5 pieces 4.7 / 5.2 / 16.7 us, 8 requests of 64 pieces 6.1 /
+  // 4.6 / 4.6, one of 512 pieces 22.9 / 8.2 / 6.0.
   const unsigned rows = (unsigned)(p.m * p.H);
   const int pieces = p.spans / p.batch;
   auto join = [&](auto pieces_) {
