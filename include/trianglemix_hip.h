@@ -501,8 +501,11 @@ int tmx_gather_dequant_kv_fp8(const void* key_cache, const void* value_cache, in
  *
  * Values: 32 neighbouring columns of a row share a power of two 2^e, stored as the byte e + 127; a value is one of 0,
  * 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, times 2^e.  The write takes e = floor(log2(amax)) - 2, one more when amax >=
- * 1.75 * 2^floor(log2(amax)), at least -126, and rounds x / 2^e to nearest, ties to the even code: nothing saturates.
- * A block with an infinity or a NaN gets the byte 255 and reads back as NaN.
+ * 1.75 * 2^floor(log2(amax)), at least -126, and rounds x / 2^e to nearest, ties to the even code: nothing saturates, but
+ * for bf16 blocks with amax >= 1.75 * 2^127, where e stays at 125 and magnitudes past 5 * 2^125 become 6 * 2^125 (the
+ * largest value of the format that bf16 and fp32 hold).  Finite rows stay finite; a block with an infinity or a NaN gets
+ * the byte 255 and reads back as NaN.  Scale bytes 253 and 254 are never written; pages from elsewhere must not hold
+ * them (their larger codes are past the range of bf16 and fp32 and would read as infinities).
  *
  * Pages: a page of page_size tokens (a power of two, at least 16) of K or of V is num_kv_heads * page_size *
  * (head_dim / 2 + head_dim / 32) bytes in one run, at page index * stride_page (bytes, a multiple of 16):

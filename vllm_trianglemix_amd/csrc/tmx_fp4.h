@@ -17,7 +17,8 @@
 
 namespace tmx {
 
-constexpr int kFp4Block = 32;  // columns per scale
+constexpr int kFp4Block = 32;          // columns per scale
+constexpr int kFp4MaxByte = 125 + 127;  // the largest scale byte that the write makes, 255 apart
 
 TMX_HD int64_t fp4_code_bytes(int kv_heads, int page_size, int head_dim) { return (int64_t)kv_heads * page_size * (head_dim / 2); }
 TMX_HD int64_t fp4_page_bytes(int kv_heads, int page_size, int head_dim) {
@@ -45,7 +46,10 @@ __device__ __forceinline__ unsigned fp4_amax8(uint4 x) {
 
 // The scale byte of a block whose largest magnitude has these 16 bits: e = floor(log2(amax)) - 2, one more from 1.75 *
 // 2^floor(log2(amax)) on.  With it amax / 2^e lies in [3.5, 7): every value of the block is within half a step of its
-// code (7 would be the midpoint above 6), none saturates.  e stays at or above -126, the smallest normal float.
+// code (7 would be the midpoint above 6), none saturates.  e stays at or above -126, the smallest normal float, and at or
+// below 125: 6 x 2^125 is the largest value a block can stand for that bf16 and fp32 hold, and what a block with amax >=
+// 1.75 x 2^127 (bf16 only) would round to otherwise is 2^128.  There the codes saturate: values past 5 x 2^125 become
+// 6 x 2^125, off by less than 2 x 2^125.
 __device__ __forceinline__ unsigned fp4_scale_byte(unsigned amax, bool bf16) {
   unsigned bits;
   if (bf16) {
@@ -56,10 +60,10 @@ __device__ __forceinline__ unsigned fp4_scale_byte(unsigned amax, bool bf16) {
   const int ex = (int)(bits >> 23);
   if (ex == 255) return 255u;
   const int e = ex - 2 + ((bits & 0x7fffffu) >= 0x600000u ? 1 : 0);
-  return (unsigned)imax(e, 1);
+  return (unsigned)imin(imax(e, 1), kFp4MaxByte);
 }
 
-// Eight 16-bit values as eight codes (the conversion instruction rounds to nearest, ties to even).  A block with scale
+// Eight 16-bit values as eight codes (the conversion instruction rounds to nearest, ties to even, and saturates at 6).  A block with scale
 // byte 255 gets zeros.
 __device__ __forceinline__ unsigned fp4_codes8(uint4 x, unsigned byte, bool bf16) {
   const float s = __uint_as_float(byte << 23);

@@ -68,8 +68,8 @@ __global__ __launch_bounds__(256) void fp4_write_kernel(
   }
 }
 
-// Eight codes as eight 16-bit values.  bf16 holds every value of the format; fp16 does not: magnitudes from 65536 on
-// saturate at 65504 (a value of 65504 is stored as 4 x 2^14), NaN stays NaN.
+// Eight codes as eight 16-bit values.  bf16 holds every value that the write makes (scale bytes up to 252); fp16 does not:
+// magnitudes from 65536 on saturate at 65504 (a value of 65504 is stored as 4 x 2^14), NaN stays NaN.
 __device__ __forceinline__ uint4 fp4_values8(unsigned w, unsigned byte, bool bf16) {
   const float s = __uint_as_float(byte << 23);
   if (bf16) return make_uint4(fp4_bf16<0>(w, s), fp4_bf16<1>(w, s), fp4_bf16<2>(w, s), fp4_bf16<3>(w, s));

@@ -840,8 +840,9 @@ def reshape_and_cache_fp4(key: torch.Tensor, value: torch.Tensor, key_cache: tor
                           slot_mapping: torch.Tensor) -> None:
     """Write this step's K/V rows ``[T, Hkv, D]`` (bf16 / fp16) into a 4-bit (MXFP4) paged cache: the counterpart of
     ``reshape_and_cache`` and ``reshape_and_cache_fp8``.  32 neighbouring columns share a power of two, values round to
-    nearest (ties to the even code); a block with an infinity or a NaN reads back as NaN.  Slots that are negative or
-    past the cache are skipped; the others must be distinct."""
+    nearest (ties to the even code; magnitudes past 5 x 2^125, which only bf16 has, to 6 x 2^125: finite rows stay finite); a
+    block with an infinity or a NaN reads back as NaN.  Slots that are negative or past the cache are skipped; the others
+    must be distinct."""
     _require_gpu(key_cache, "key_cache")
     C = _op_binding()
     if C is not None:
