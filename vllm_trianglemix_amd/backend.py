@@ -210,6 +210,19 @@ class TriangleMixAttentionMetadata:
             self._workspaces[key] = ws
         return ws
 
+    def decode_fp4_workspace(self, batch: int, rows: int, num_heads: int, num_kv_heads: int, head_size: int, device) -> tuple:
+        """Work area of the launch that reads a 4-bit cache in place, for ``batch`` requests of ``rows`` rows.  A step that
+        is captured takes the builder's, which is kept; any other one has its own, shared by its layers and gone with
+        the step: the sizes that come up while serving (batch sizes x drafted rows; 26 MB for 64 requests of 8 rows and 64
+        heads, 11 GB for all of 1 to 256 requests) do not add up."""
+        if self.builder is not None and (self.capturing or (device.type == "cuda" and torch.cuda.is_current_stream_capturing())):
+            return self.builder.decode_fp4_workspace(batch, rows, num_heads, num_kv_heads, head_size)
+        key = ("fp4", batch, rows, num_heads, num_kv_heads, head_size)
+        ws = self._workspaces.get(key)
+        if ws is None:
+            ws = self._workspaces[key] = ops.decode_fp4_workspace(batch, rows, num_heads, num_kv_heads, head_size, device)
+        return ws
+
 
 # How the step's K/V rows reach the 16-bit paged cache (TRIANGLEMIX_CACHE_WRITE):
 #   "fused"  (default) the attention launch stores them itself (cache_slots) and reads the step's keys from the
@@ -273,7 +286,7 @@ class TriangleMixMetadataBuilder(_BuilderBase):
         return ws
 
     def decode_fp4_workspace(self, batch: int, rows: int, num_heads: int, num_kv_heads: int, head_size: int) -> tuple:
-        """The same for the launch that reads a 4-bit cache, per batch size and rows per request."""
+        """The same for captured launches that read a 4-bit cache, per batch size and rows per request."""
         key = ("fp4", batch, rows, num_heads, num_kv_heads, head_size)
         ws = self._decode_ws.get(key)
         if ws is None:
@@ -595,11 +608,7 @@ class TriangleMixAttentionImpl(_ImplBase):
                                       m.slot_mapping[:n_tok])
         rows = self._fp4_rows_in_place(m)
         if rows:
-            batch = n_tok // rows
-            if m.builder is not None:
-                ws = m.builder.decode_fp4_workspace(batch, rows, self.num_heads, self.num_kv_heads, self.head_size)
-            else:
-                ws = ops.decode_fp4_workspace(batch, rows, self.num_heads, self.num_kv_heads, self.head_size, q.device)
+            ws = m.decode_fp4_workspace(n_tok // rows, rows, self.num_heads, self.num_kv_heads, self.head_size, q.device)
             ops.decode_attention_fp4(q, key_cache, value_cache, out, m.block_table, m.seq_lens, self.scale, ws,
                                      rows_per_request=rows)
             return output
