@@ -1,4 +1,4 @@
-"""The 4-bit cache behind the backend: which memory its steps keep."""
+"""The 4-bit cache behind the backend: which memory its steps keep, and mixed steps (running requests beside prompts)."""
 import gc
 import types
 import weakref
@@ -7,6 +7,8 @@ import numpy as np
 import pytest
 import torch
 
+import fp4_reference as ref
+from vllm_trianglemix_amd import backend as be
 from vllm_trianglemix_amd import ops
 from vllm_trianglemix_amd.backend import TriangleMixAttentionBackend as B
 
@@ -45,6 +47,15 @@ class Recorder:
         monkeypatch.setattr(ops, "reshape_and_cache_fp4", lambda *a: self.calls.append(("write", *a)))
         monkeypatch.setattr(ops, "decode_attention_fp4", lambda *a, rows_per_request: self.calls.append(("in place", rows_per_request, *a)))
 
+        monkeypatch.setattr(ops, "gather_dequant_kv_fp4", self.gather)
+        monkeypatch.setattr(ops, "attention", lambda *a, **kw: self.calls.append(("over rows", *a)))
+        monkeypatch.setattr(be.TriangleMixAttentionMetadata, "block_index", lambda m, *a, **kw: m)
+        monkeypatch.setattr(be.TriangleMixAttentionMetadata, "workspace", lambda m, *a: None)
+
+    def gather(self, k, v, table, lens, cu, total, longest, dtype):
+        self.calls.append(("read back", table, lens, cu, total, longest))
+        return torch.empty(0), torch.empty(0)
+
     def area(self, batch, rows, num_heads, num_kv_heads, head_dim, device):
         t = torch.empty(1), torch.empty(1)
         self.areas.append(weakref.ref(t[0]))
@@ -81,6 +92,155 @@ def test_work_areas_of_served_steps_do_not_add_up(monkeypatch):
         step(builder.build(0, common([1] * batch, [40] * batch)))
     assert kept() is not None
     assert step(builder.build_for_cudagraph_capture(common([1] * 4, [40] * 4)))() is kept()
+
+
+def mixed(rec, builder, impl, q_lens, seq_lens, prompts=None):
+    """The calls of a step: (requests, rows of each) in place, (row offsets, lengths) of those over rows read back."""
+    T = sum(q_lens)
+    table = torch.arange(len(q_lens), dtype=torch.int32).view(-1, 1)
+    m = builder.build(0, common(q_lens, seq_lens, table, torch.arange(T), prompts=prompts))
+    H, D, Hkv = impl.num_heads, impl.head_size, impl.num_kv_heads
+    q = torch.arange(T, dtype=torch.float32).view(-1, 1).expand(T, H * D).contiguous()
+    k = torch.zeros(T, Hkv * D)
+    out = -q
+    kv = torch.zeros(B.get_kv_cache_shape(4, 16, Hkv, D, "mxfp4"), dtype=torch.uint8)
+    rec.calls.clear()
+    impl.forward(None, q, k, k, kv, m, out)
+    calls = {c[0]: c[1:] for c in rec.calls}
+    assert calls["write"][4].tolist() == list(range(T))
+    place = back = None
+    at = 0
+    if "in place" in calls:
+        rows, cq, _, _, cout, ctable, clens = calls["in place"][:7]
+        n = cq.shape[0] // rows
+        place = n, rows
+        assert cq[:, 0, 0].tolist() == list(range(n * rows)) == [-x for x in cout[:, 0, 0].tolist()]
+        assert ctable[:n, 0].tolist() == list(range(n)) and clens[:n].tolist() == seq_lens[:n]
+        at = n
+    if "read back" in calls:
+        rtable, lens, cu, total, longest = calls["read back"]
+        aq, _, _, aout, rest, acu, alens = calls["over rows"][:7]
+        first = sum(q_lens[:at])
+        back = (acu.tolist(), lens.tolist())
+        assert rtable[:, 0].tolist() == list(range(at, len(q_lens)))
+        assert lens.tolist() == alens.tolist() == seq_lens[at:] == rest.seq_lens_cpu.tolist()
+        assert acu.tolist() == np.concatenate([[0], np.cumsum(q_lens[at:])]).tolist() == rest.query_start_loc_cpu.tolist()
+        assert cu.tolist() == np.concatenate([[0], np.cumsum(seq_lens[at:])]).tolist() and total == sum(seq_lens[at:]) and longest >= max(seq_lens[at:])
+        assert aq[:, 0, 0].tolist() == list(range(first, T)) == [-x for x in aout[:, 0, 0].tolist()]
+        assert rest.slot_mapping.tolist() == list(range(first, T)) and rest.num_actual_tokens == T - first
+        assert rest.max_query_len == max(q_lens[at:])
+        assert (rest.prompt_lens_cpu is None) == (prompts is None)
+        if prompts is not None:
+            assert rest.prompt_lens_cpu.tolist() == prompts[at:] == rest.prompt_lens.tolist()
+    assert at * (place or (0, 0))[1] + (0 if back is None else back[0][-1]) == T
+    return place, back
+
+
+def test_requests_beside_a_prompt_are_not_read_back(monkeypatch):
+    """A step of running requests and a chunk of a prompt: the cached rows of the former stay in 4 bits."""
+    rec, builder = Recorder(monkeypatch), builder_for("cpu")
+    causal, tri = layer(8, 128, 2, use_triangle=False), layer(8, 128, 2, use_triangle=True, num_last_tokens=4)
+    long = [60000, 30000, 40000]  # 133 MB as 16-bit rows of 2 heads
+    for impl in (causal, tri):
+        place, back = mixed(rec, builder, impl, [1, 1, 1, 300], long + [700])
+        assert place == (3, 1) and back == ([0, 300], [700])
+        place, back = mixed(rec, builder, impl, [3, 3, 3, 1, 300], long + [9, 700])
+        assert place == (3, 3) and back == ([0, 1, 301], [9, 700])
+        assert mixed(rec, builder, impl, [300, 1, 1, 1], [700] + long)[0] is None  # (no running request at the beginning)
+        assert mixed(rec, builder, impl, [1, 1, 300], [500, 40, 700])[0] is None  # little to read back: one call
+        assert mixed(rec, builder, impl, [17, 17, 300], long)[0] is None  # 68 rows per K/V head
+    # a triangle layer: rows past the trailing dense ones, and prompts that are not complete
+    assert mixed(rec, builder, tri, [4, 4, 300], long)[0] is None and mixed(rec, builder, causal, [4, 4, 300], long)[0] == (2, 4)
+    assert mixed(rec, builder, tri, [1, 1, 1, 9], long + [30], [60000, 30000, 50000, 30])[0] == (2, 1)
+    assert mixed(rec, builder, causal, [1, 1, 1, 9], long + [30], [60000, 30000, 50000, 30])[0] == (3, 1)
+    assert mixed(rec, builder, tri, [1, 1, 9], long, [60001, 30000, 40000])[0] is None
+    # the switch that keeps decode requests on the block index keeps these too
+    monkeypatch.setattr(be, "_DECODE_FIXED", False)
+    assert mixed(rec, builder, causal, [1, 1, 1, 300], long + [700])[0] is None
+
+
+def test_the_layers_of_a_mixed_step_share_its_second_part(monkeypatch):
+    builder = builder_for("cpu")
+    m = builder.build(0, common([1, 1, 30], [50, 60, 70]))
+    assert m.after(2) is m.after(2) and m.after(1) is not m.after(2)
+    assert m.leading_requests(1) == (2, 1) and m.leading_requests(0) == (0, 0)
+    padded = builder.build(0, common([1, 1, 30], [50, 60, 70]))
+    padded.num_actual_tokens = 40
+    assert padded.leading_requests(4) == (0, 0)
+
+
+def test_the_runner_is_asked_for_decode_requests_first():
+    mx = builder_for("cpu", cache_config=types.SimpleNamespace(cache_dtype="mxfp4"))
+    assert mx.reorder_batch_threshold == 1
+    assert builder_for("cpu", cache_config=types.SimpleNamespace(cache_dtype="fp8")).reorder_batch_threshold is None
+    assert builder_for("cpu").reorder_batch_threshold is None and B.get_builder_cls().reorder_batch_threshold is None
+
+
+@gpu
+@pytest.mark.parametrize("dtype, D, H, Hkv", [(torch.bfloat16, 128, 8, 2), (torch.float16, 64, 4, 2)])
+@pytest.mark.parametrize("use_triangle", [True, False])
+def test_mixed_steps_against_the_formula(monkeypatch, dtype, D, H, Hkv, use_triangle):
+    from oracle import trianglemix_oracle as orc
+    from parity_tolerance import assert_close
+    monkeypatch.setattr(be, "_FP4_SPLIT_BYTES", 0)
+    rng = np.random.default_rng(8)
+    page, gate, si, sl, last = 16, 64, 4, 32, 16
+    impl = layer(H, D, Hkv, use_triangle=use_triangle, num_sink_tokens=si, sliding_window_size=sl, num_last_tokens=last,
+                 short_sequence_gate=gate)
+    builder = builder_for(DEV)
+    for q_lens, seq_lens, prompts, split in (
+            ([1, 1, 40], [300, 17, 40], None, (2, 1)), ([1, 1, 1, 100, 3], [33, 500, 1, 180, 90], None, (3, 1)),
+            ([3, 3, 70, 1], [200, 3, 150, 64], None, (2, 3)), ([1, 80, 1], [129, 200, 90], [100, 400, 90], (1, 1)),
+            ([2, 2, 50], [120, 70, 90], [200, 70, 90], (0, 0) if use_triangle else (2, 2)), ([50, 1, 1], [60, 200, 300], None, (0, 0)),
+            ([1, 1, 1, 17], [1, 2, 3, 17], None, (3, 1))):
+        T, R = sum(q_lens), len(q_lens)
+        width = max(-(-n // page) for n in seq_lens)
+        table = rng.permutation(R * width).astype(np.int32).reshape(R, width)
+        held = [[rng.standard_normal((n, Hkv, D)) for _ in range(2)] for n in seq_lens]
+        held = [[torch.from_numpy(x).to(dtype) for x in pair] for pair in held]
+        kv = torch.zeros(B.get_kv_cache_shape(R * width, page, Hkv, D, "mxfp4"), dtype=torch.uint8, device=DEV)
+        slots = [table[r, np.arange(n) // page].astype(np.int64) * page + np.arange(n) % page for r, n in enumerate(seq_lens)]
+        for r, (n, m) in enumerate(zip(seq_lens, q_lens)):
+            if n > m:
+                ops.reshape_and_cache_fp4(held[r][0][:n - m].to(DEV), held[r][1][:n - m].to(DEV), kv[0], kv[1], torch.from_numpy(slots[r][:n - m]).to(DEV))
+        q = torch.from_numpy(rng.standard_normal((T, H, D))).to(dtype)
+        new = [torch.cat([h[x][n - m:] for h, n, m in zip(held, seq_lens, q_lens)]).view(T, -1).to(DEV) for x in range(2)]
+        c = common(q_lens, seq_lens, torch.from_numpy(table).to(DEV),
+                   torch.from_numpy(np.concatenate([s[n - m:] for s, n, m in zip(slots, seq_lens, q_lens)])).to(DEV), DEV, prompts)
+        md = builder.build(0, c)
+        assert impl._fp4_leading_requests(md) == split
+        out = torch.zeros(T, H * D, dtype=dtype, device=DEV)
+        impl.forward(None, q.to(DEV).view(T, -1), *new, kv, md, out)
+        got, at = out.view(T, H, D).double().cpu().numpy(), 0
+        for r, (n, m) in enumerate(zip(seq_lens, q_lens)):
+            full = n if prompts is None else max(n, prompts[r])
+            kd, vd = (ref.values(*ref.quantise(x.double().numpy())) for x in held[r])
+            kw = dict(full_lens=[full]) if full != n else {}
+            want = orc.varlen_gqa_attention(q[at:at + m].double().numpy(), lambda b: kd, lambda b: vd, [0, m], [n], D ** -0.5,
+                                            "triangle" if use_triangle and full > gate else "causal", si, sl, last, **kw)
+            assert_close(got[at:at + m], want, "backend forward, 4-bit cache, mixed steps", out16=True)
+            at += m
+
+
+@gpu
+def test_memory_of_a_mixed_step():
+    """32 requests of 2000 cached tokens beside a short prompt: nothing of the size of their 16-bit rows is allocated."""
+    H, D, Hkv, page, n, R = 8, 128, 2, 16, 2000, 32
+    builder, impl = builder_for(DEV), layer(H, D, Hkv, use_triangle=False)
+    width = n // page
+    kv = torch.zeros(B.get_kv_cache_shape((R + 1) * width, page, Hkv, D, "mxfp4"), dtype=torch.uint8, device=DEV)
+    table = torch.arange((R + 1) * width, dtype=torch.int32, device=DEV).view(R + 1, width)
+    T = R + 40
+    c = common([1] * R + [40], [n] * R + [40], table, torch.full((T,), -1, dtype=torch.int64, device=DEV), DEV)
+    q, k = torch.zeros(T, H * D, dtype=torch.bfloat16, device=DEV), torch.zeros(T, Hkv * D, dtype=torch.bfloat16, device=DEV)
+    out = torch.zeros_like(q)
+    impl.forward(None, q, k, k, kv, builder.build(0, c), out)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    impl.forward(None, q, k, k, kv, builder.build(0, c), out)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < 4 * R * n * Hkv * D // 4
 
 
 @gpu

@@ -188,6 +188,35 @@ class TriangleMixAttentionMetadata:
         rows of its pattern)."""
         return self.prompt_lens_cpu is None or bool(np.all(self.prompt_lens_cpu <= self.seq_lens_cpu))
 
+    def leading_requests(self, most_rows: int) -> Tuple[int, int]:
+        """The requests at the step's beginning that have one number of query rows, at most ``most_rows``: (how many, rows
+        of each), (0, 0) when the first one has more."""
+        q = np.diff(self.query_start_loc_cpu)
+        if q.shape[0] != self.seq_lens_cpu.shape[0] or q.shape[0] == 0 or int(self.query_start_loc_cpu[-1]) != self.num_actual_tokens:
+            return 0, 0
+        rows = int(q[0])
+        if not 1 <= rows <= most_rows:
+            return 0, 0
+        others = np.flatnonzero(q != rows)
+        return (int(others[0]) if others.size else q.shape[0]), rows
+
+    def after(self, count: int) -> "TriangleMixAttentionMetadata":
+        """The step without its first ``count`` requests (their rows aside, the first of the others is row 0): made once
+        per step, shared by the layers."""
+        rest = self.__dict__.setdefault("_after", {}).get(count)
+        if rest is None:
+            first = int(self.query_start_loc_cpu[count])
+            cu, sl = self.query_start_loc_cpu[count:] - np.int32(first), self.seq_lens_cpu[count:]
+            end = self.seq_lens_cpu.shape[0]
+            rest = self.__dict__["_after"][count] = TriangleMixAttentionMetadata(
+                num_actual_tokens=self.num_actual_tokens - first, max_query_len=int(np.diff(cu).max()),
+                query_start_loc=self.query_start_loc[count:] - first, max_seq_len=int(sl.max()), seq_lens=self.seq_lens[count:end],
+                block_table=self.block_table[count:end], slot_mapping=self.slot_mapping[first:], query_start_loc_cpu=cu,
+                seq_lens_cpu=sl, page_size=self.page_size,
+                prompt_lens=None if self.prompt_lens is None else self.prompt_lens[count:],
+                prompt_lens_cpu=None if self.prompt_lens_cpu is None else self.prompt_lens_cpu[count:], builder=self.builder)
+        return rest
+
     def fp8_row_offsets(self, device):
         """Row offsets of every request's keys in a contiguous copy of the step's K/V (``cu_seqlens_k``), on the
         device, and their total: made once per step, shared by the layers."""
@@ -235,6 +264,11 @@ _CACHE_WRITE_STREAM = os.environ.get("TRIANGLEMIX_CACHE_WRITE_STREAM", "1") != "
 # Steps of one-row requests take the launch with a fixed shape (no index, nothing sized on the host from the
 # lengths; the only form that replays under a graph).  "0": they go through the block index like every other step.
 _DECODE_FIXED = os.environ.get("TRIANGLEMIX_DECODE_FIXED", "1") != "0"
+# A mixed step out of a 4-bit cache is split (the requests it begins with in place, the others over rows read back) from this
+# many bytes of 16-bit rows on: the second call costs 12 to 16 us a layer on the host.  Requests beside a prompt of 64 / 512
+# rows, 8 K/V heads of 128, us a layer without / with the split: 4 x 2048 keys (34 MB) 59.9 / 71.9, 16 x 1024 (67 MB) 93.2 /
+# 71.4; beside 2048 rows of a prompt of 8192, 64 x 8192 keys (2.1 GB) 1075 / 336.
+_FP4_SPLIT_BYTES = 48 << 20
 _side_streams: Dict[int, "torch.cuda.Stream"] = {}
 
 
@@ -275,6 +309,9 @@ class TriangleMixMetadataBuilder(_BuilderBase):
         self.device = device
         self.block_size = int(kv_cache_spec.block_size)
         self._decode_ws: Dict[Tuple, tuple] = {}
+        if getattr(getattr(vllm_config, "cache_config", None), "cache_dtype", None) == "mxfp4":
+            # decode requests first in every step: the layers read a 4-bit cache in place for the requests a step begins with
+            self.reorder_batch_threshold = 1
 
     def decode_workspace(self, batch: int, num_heads: int, num_kv_heads: int, head_size: int, fp8: bool) -> tuple:
         """Work area of the fixed-shape decode launch for a batch size, held for the builder's life: a captured
@@ -596,8 +633,8 @@ class TriangleMixAttentionImpl(_ImplBase):
 
     def _forward_fp4_cache(self, q, key, value, key_cache, value_cache, m, output):
         """kv_cache_dtype "mxfp4": the step's rows are quantised into the pages, and the attention reads what the pages
-        hold -- in place for steps whose requests all have the same few rows (decode, drafted tokens), through 16-bit
-        rows read back for the step otherwise (prompts)."""
+        hold -- in place for steps whose requests all have the same few rows (decode, drafted tokens) and for the requests
+        at a step's beginning that do, through 16-bit rows read back for the step otherwise (prompts)."""
         n_tok = m.num_actual_tokens
         out = output.view(-1, self.num_heads, self.head_size)[:n_tok]
         if n_tok == 0:
@@ -608,12 +645,29 @@ class TriangleMixAttentionImpl(_ImplBase):
                                       m.slot_mapping[:n_tok])
         rows = self._fp4_rows_in_place(m)
         if rows:
-            ws = m.decode_fp4_workspace(n_tok // rows, rows, self.num_heads, self.num_kv_heads, self.head_size, q.device)
-            ops.decode_attention_fp4(q, key_cache, value_cache, out, m.block_table, m.seq_lens, self.scale, ws,
-                                     rows_per_request=rows)
+            self._fp4_in_place(q, key_cache, value_cache, m, out, rows)
             return output
         if m.capturing:
             raise NotImplementedError("this layer has no decode launch that replays under a graph (num_last_tokens >= 2)")
+        count, rows = self._fp4_leading_requests(m)
+        if count:
+            # Their context -- all of the running sequences', beside a chunk of one prompt -- is not read back.
+            split = count * rows
+            self._fp4_in_place(q[:split], key_cache, value_cache, m, out[:split], rows)
+            if split == n_tok:
+                return output
+            q, out, m = q[split:], out[split:], m.after(count)
+        self._fp4_read_back(q, key_cache, value_cache, m, out)
+        return output
+
+    def _fp4_in_place(self, q, key_cache, value_cache, m, out, rows):
+        """The first ``q.shape[0] / rows`` requests of the step, each with ``rows`` rows."""
+        ws = m.decode_fp4_workspace(q.shape[0] // rows, rows, self.num_heads, self.num_kv_heads, self.head_size, q.device)
+        ops.decode_attention_fp4(q, key_cache, value_cache, out, m.block_table, m.seq_lens, self.scale, ws, rows_per_request=rows)
+
+    def _fp4_read_back(self, q, key_cache, value_cache, m, out):
+        """All requests of the step over their keys and values as 16-bit rows, which take 4 x keys x K/V heads x head size
+        bytes while the layer runs."""
         mode = "triangle" if self.use_triangle else "causal"
         pattern = self.pattern if self.use_triangle else (0, 0, 0)
         tri_min_len = self.tri_min_len if self.use_triangle else 0
@@ -624,7 +678,28 @@ class TriangleMixAttentionImpl(_ImplBase):
                                                    int(m.max_seq_len), q.dtype)
         ops.attention(q, k_rows, v_rows, out, idx, m.query_start_loc, m.seq_lens, self.scale, cu_seqlens_k=cu_k,
                       workspace=ws, flags=_step_flags(m))
-        return output
+
+    def _fp4_leading_requests(self, m) -> Tuple[int, int]:
+        """The requests at the beginning of a mixed step that the in-place launch takes, and their rows; (0, 0) without any.
+        The rule of :meth:`_fp4_rows_in_place`, request by request, where reading them back would take
+        ``_FP4_SPLIT_BYTES`` or more."""
+        if not _DECODE_FIXED:
+            return 0, 0
+        most = 64 // (self.num_heads // self.num_kv_heads)
+        if self.use_triangle:
+            most = min(most, self.pattern[2] - 1)
+        key = (most, self.use_triangle, self.num_kv_heads * self.head_size)
+        hit = m.__dict__.setdefault("_fp4_leading", {}).get(key)
+        if hit is None:
+            count, rows = m.leading_requests(most)
+            if count and self.use_triangle and m.prompt_lens_cpu is not None:
+                coming = np.flatnonzero(m.prompt_lens_cpu[:count] > m.seq_lens_cpu[:count])
+                if coming.size:
+                    count = int(coming[0])
+            if 4 * int(m.seq_lens_cpu[:count].sum(dtype=np.int64)) * key[2] < _FP4_SPLIT_BYTES:
+                count = 0
+            hit = m.__dict__["_fp4_leading"][key] = (count, rows) if count else (0, 0)
+        return hit
 
     def _fp4_rows_in_place(self, m) -> int:
         """Rows per request of a step that the in-place launch covers, 0 for others.  It attends to every key up to a
