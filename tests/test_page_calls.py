@@ -1,0 +1,102 @@
+"""How the page operators' calls reach the library: as plain functions of the extension, or through the registry where
+something is to see them; what they refuse."""
+import warnings
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.overrides import TorchFunctionMode
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from vllm_trianglemix_amd import _lib, ops, torch_ops
+
+gpu = pytest.mark.gpu
+DEV = "cuda:0"
+NAMES = ["trianglemix_free_pages", "trianglemix_fork_pages", "trianglemix_copy_pages", "trianglemix_compact_pages"]
+
+
+def inputs():
+    caches = [(torch.arange(12 * 64, device=DEV) % 251 + i).to(torch.uint8).view(12, 64) for i in range(3)]
+    table = torch.tensor([[9, 3, -1], [7, 9, 11]], dtype=torch.int32, device=DEV)
+    return caches, table, torch.tensor([20, 41], dtype=torch.int32, device=DEV)
+
+
+def all_four(caches, table, lens):
+    free, n = ops.free_pages(table, lens, 12, 16)
+    child = ops.fork_pages(caches, table, lens, torch.tensor([1, 0], dtype=torch.int32, device=DEV), free[:2], 16)
+    ops.copy_pages(caches, torch.tensor([[9, 5], [11, 6]], device=DEV))
+    new, used = ops.compact_pages(caches, table, lens, 16)
+    return [free, n, child, new, used, *caches]
+
+
+def test_fake_tensors_never_reach_the_library():
+    """They have no memory: nothing may take their address, whether a device is there or not.  The registry answers for them:
+    a call without results is traced, the others say that they have no fake form."""
+    with FakeTensorMode(), warnings.catch_warnings():
+        warnings.simplefilter("error")
+        caches, table, lens = inputs()
+        assert ops.copy_pages(caches, table[:, :2].long().contiguous()) is None
+        for call in (lambda: ops.free_pages(table, lens, 12, 16), lambda: ops.fork_pages(caches, table, lens, lens, lens, 16),
+                     lambda: ops.compact_pages(caches, table, lens, 16), lambda: ops.compact_pages(tuple(caches), table, lens, 16)):
+            with pytest.raises(_lib.TmxError, match="trianglemix_(free|fork|compact)_pages"):
+                call()
+
+
+def test_the_number_of_arguments_is_checked():
+    torch_ops.load()
+    t = torch.zeros(1, 2, dtype=torch.int64)
+    m = torch_ops.module
+    for f, right in ((m.copy_pages, 2), (m.free_pages, 4), (m.compact_pages, 4), (m.fork_pages, 6)):
+        for n in (0, right - 1, right + 1):
+            with pytest.raises(RuntimeError, match=f"takes {right} arguments"):
+                f(*[t] * n)
+
+
+@gpu
+def test_modes_and_profilers_see_the_calls():
+    want = all_four(*inputs())
+    seen = []
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func.__name__)
+            return func(*args, **(kwargs or {}))
+
+    class Function(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(getattr(func, "__name__", ""))
+            return func(*args, **(kwargs or {}))
+
+    for mode in (Dispatch, Function):
+        seen.clear()
+        with mode():
+            got = all_four(*inputs())
+        assert [n.split(".")[0] for n in seen if "pages" in n] == NAMES
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        got = all_four(*inputs())
+    names = [e.name for e in prof.events()]
+    assert all(any(n.endswith(x) for n in names) for x in NAMES)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # and a subclass of Tensor
+    class Mine(torch.Tensor):
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            seen.append(getattr(func, "__name__", ""))
+            return super().__torch_function__(func, types, args, kwargs or {})
+
+    seen.clear()
+    caches, table, lens = inputs()
+    ops.copy_pages([caches[0].as_subclass(Mine), *caches[1:]], torch.tensor([[9, 5]], device=DEV))
+    assert any(n.startswith("trianglemix_copy_pages") for n in seen) and torch.equal(caches[0][9], caches[0][5])
+
+
+@gpu
+def test_plain_calls_stay_plain():
+    caches, table, lens = inputs()
+    m = torch_ops.module
+    assert m.free_pages(table, lens, 12, 16) is not NotImplemented
+    with torch.inference_mode():
+        assert m.copy_pages(caches, torch.tensor([[9, 5]], device=DEV)) is None
+    with torch.no_grad():
+        assert m.compact_pages(caches, table, lens, 16) is not NotImplemented

@@ -729,26 +729,44 @@ TORCH_LIBRARY(_trianglemix_C, m) {
 // The extension is also a Python module, so that a plain `import` of the shared object runs the
 // TORCH_LIBRARY block above: the reference's REGISTER_EXTENSION (csrc/core/registration.h:13-27), which is
 // how vllm/platforms/rocm.py:32-40 loads vllm._C / vllm._rocm_C.
+#include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/record_function.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 // The page operators are also plain functions of the module (same names without the prefix, positional arguments): turning
 // a Python list of 72 tensors into the registry's own costs 5.2 us of a call's 10.7, reading it in place 0.2 us, and outputs
 // made below the autograd keys, as in the registry's kernels, are handed to Python as they are (free_pages 6.2 -> 4.8 us).
-// (Calls that only fill their arguments gain nothing: they stay with the registry.)
+// (Calls that only fill their arguments gain nothing: they stay with the registry.)  They serve plain tensors that nothing
+// watches.  With a dispatch or function mode, a tensor subclass (a fake tensor has no memory to work on), a functorch
+// transform or a profiler about, they do nothing and return NotImplemented: the caller then goes through the registry, which
+// these see.
 namespace {
+
+const c10::DispatchKeySet kWatchers(
+    {c10::DispatchKey::Python, c10::DispatchKey::PythonDispatcher, c10::DispatchKey::Functionalize, c10::DispatchKey::Tracer,
+     c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchVmapMode, c10::DispatchKey::FuncTorchGradWrapper,
+     c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchDynamicLayerBackMode});
 
 struct Args {
   PyObject* const* at;
   Py_ssize_t n, next = 0;
-  PyObject* take() {
-    TORCH_CHECK(next < n, "trianglemix: too few arguments");
-    return at[next++];
+  bool watched = at::hasCallbacks() || at::impl::torch_function_mode_enabled() ||
+                 c10::impl::tls_local_dispatch_key_set().included_.has_any(kWatchers);
+  Args(PyObject* const* at, Py_ssize_t n, Py_ssize_t takes) : at(at), n(n) {
+    TORCH_CHECK(n == takes, "trianglemix: the operator takes ", takes, " arguments, not ", n);
+  }
+  PyObject* take() { return at[next++]; }
+  const Tensor& variable(PyObject* o) {
+    const Tensor& t = THPVariable_Unpack(o);
+    watched = watched || t.key_set().has_any(kWatchers) || !THPVariable_CheckExact(o);
+    return t;
   }
   const Tensor& tensor() {
     PyObject* o = take();
     TORCH_CHECK(THPVariable_Check(o), "trianglemix: argument ", next, " must be a tensor");
-    return THPVariable_Unpack(o);
+    return variable(o);
   }
   int64_t integer() {
     PyObject* o = take();
@@ -765,7 +783,7 @@ struct Args {
     r.reserve((size_t)k);
     for (Py_ssize_t i = 0; i < k; ++i) {
       TORCH_CHECK(THPVariable_Check(items[i]), "trianglemix: argument ", next, " must hold tensors only");
-      r.push_back(&THPVariable_Unpack(items[i]));
+      r.push_back(&variable(items[i]));
     }
     return r;
   }
@@ -782,37 +800,44 @@ PyObject* two(const std::tuple<Tensor, Tensor>& t) {
 
 PyObject* py_copy_pages(PyObject*, PyObject* const* at, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  Args a{at, n};
+  Args a{at, n, 2};
   const TensorRefs caches = a.tensors();
-  copy_pages(caches, a.tensor());
+  const Tensor& pairs = a.tensor();
+  if (a.watched) Py_RETURN_NOTIMPLEMENTED;
+  copy_pages(caches, pairs);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
 PyObject* py_fork_pages(PyObject*, PyObject* const* at, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  const at::AutoDispatchBelowADInplaceOrView below;
-  Args a{at, n};
+  Args a{at, n, 6};
   const TensorRefs caches = a.tensors();
   const Tensor &bt = a.tensor(), &sl = a.tensor(), &parents = a.tensor(), &fresh = a.tensor();
-  return THPVariable_Wrap(fork_pages(caches, bt, sl, parents, fresh, a.integer()));
+  const int64_t page_size = a.integer();
+  if (a.watched) Py_RETURN_NOTIMPLEMENTED;
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return THPVariable_Wrap(fork_pages(caches, bt, sl, parents, fresh, page_size));
   END_HANDLE_TH_ERRORS
 }
 PyObject* py_free_pages(PyObject*, PyObject* const* at, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  const at::AutoDispatchBelowADInplaceOrView below;
-  Args a{at, n};
+  Args a{at, n, 4};
   const Tensor &bt = a.tensor(), &sl = a.tensor();
-  const int64_t pages = a.integer();
-  return two(free_pages(bt, sl, pages, a.integer()));
+  const int64_t pages = a.integer(), page_size = a.integer();
+  if (a.watched) Py_RETURN_NOTIMPLEMENTED;
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return two(free_pages(bt, sl, pages, page_size));
   END_HANDLE_TH_ERRORS
 }
 PyObject* py_compact_pages(PyObject*, PyObject* const* at, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  const at::AutoDispatchBelowADInplaceOrView below;
-  Args a{at, n};
+  Args a{at, n, 4};
   const TensorRefs caches = a.tensors();
   const Tensor &bt = a.tensor(), &sl = a.tensor();
-  return two(compact_pages(caches, bt, sl, a.integer()));
+  const int64_t page_size = a.integer();
+  if (a.watched) Py_RETURN_NOTIMPLEMENTED;
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return two(compact_pages(caches, bt, sl, page_size));
   END_HANDLE_TH_ERRORS
 }
 

@@ -829,6 +829,13 @@ def _call(op, *args):
         raise _lib.TmxError(-1, str(e)) from None
 
 
+def _page_call(module, name: str, *args):
+    """A page operator as a plain function of the extension; through the registry where something is to see the call (a
+    dispatch mode, a tensor subclass such as a fake tensor, a profiler)."""
+    r = _call(getattr(module, name), *args)
+    return r if r is not NotImplemented else _call(getattr(_op_binding(), "trianglemix_" + name).default, *args)
+
+
 def _on(device: torch.device, *tensors) -> None:
     for t, name in tensors:
         _require_gpu(t, name)
@@ -1027,7 +1034,7 @@ def copy_pages(caches: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
     _require_gpu(pairs, "pairs")
     C = _module()
     if C is not None:
-        _call(C.copy_pages, caches, pairs)
+        _page_call(C, "copy_pages", caches, pairs)
         return
     dev = pairs.device
     at, size, stride, pages = _page_list(caches, dev)
@@ -1045,7 +1052,7 @@ def free_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, num_pages: int
     _require_gpu(block_table, "block_table")
     C = _module()
     if C is not None:
-        return _call(C.free_pages, block_table, seq_lens, int(num_pages), int(page_size))
+        return _page_call(C, "free_pages", block_table, seq_lens, int(num_pages), int(page_size))
     dev = _page_table(block_table, seq_lens)
     if num_pages < 0:
         raise RuntimeError("num_pages must not be negative")
@@ -1069,7 +1076,7 @@ def fork_pages(caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq_le
     _require_gpu(block_table, "block_table")
     C = _module()
     if C is not None:
-        return _call(C.fork_pages, caches, block_table, seq_lens, parents, fresh, int(page_size))
+        return _page_call(C, "fork_pages", caches, block_table, seq_lens, parents, fresh, int(page_size))
     dev = _page_table(block_table, seq_lens)
     at, size, stride, pages = _page_list(caches, dev)
     _on(dev, (parents, "parents"), (fresh, "fresh"))
@@ -1092,7 +1099,7 @@ def compact_pages(caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq
     _require_gpu(block_table, "block_table")
     C = _module()
     if C is not None:
-        return _call(C.compact_pages, caches, block_table, seq_lens, int(page_size))
+        return _page_call(C, "compact_pages", caches, block_table, seq_lens, int(page_size))
     dev = _page_table(block_table, seq_lens)
     if not len(caches):
         raise RuntimeError("compact_pages needs the caches (their first dimension is the pool)")
