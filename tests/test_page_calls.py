@@ -52,6 +52,25 @@ def test_the_number_of_arguments_is_checked():
                 f(*[t] * n)
 
 
+@pytest.mark.parametrize("error, comes_as", [
+    (torch.OutOfMemoryError, torch.OutOfMemoryError), (torch.AcceleratorError, torch.AcceleratorError), (RuntimeError, _lib.TmxError),
+    (NotImplementedError, _lib.TmxError), (TypeError, _lib.TmxError), (KeyboardInterrupt, KeyboardInterrupt)])
+def test_which_errors_are_refusals(monkeypatch, error, comes_as):
+    """Callers tell memory that has run out (which they may free and try again) from arguments that are refused."""
+    def raises(*args):
+        raise error("what happened")
+
+    torch_ops.load()
+    monkeypatch.setattr(ops, "_require_gpu", lambda t, name: None)
+    monkeypatch.setattr(torch_ops, "module", type("Module", (), dict.fromkeys(("free_pages", "copy_pages", "fork_pages", "compact_pages"), staticmethod(raises))))
+    t = torch.zeros(1, 2, dtype=torch.int32)
+    for call in (lambda: ops.free_pages(t, t, 8, 16), lambda: ops.copy_pages([t], t), lambda: ops.fork_pages([t], t, t, t, t, 16),
+                 lambda: ops.compact_pages([t], t, t, 16)):
+        with pytest.raises(comes_as) as e:
+            call()
+        assert type(e.value) is comes_as
+
+
 @gpu
 def test_modes_and_profilers_see_the_calls():
     want = all_four(*inputs())

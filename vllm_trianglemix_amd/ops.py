@@ -822,9 +822,12 @@ def _module():
 
 
 def _call(op, *args):
-    """A call of the extension: its refusals come as TmxError, like the library's own."""
+    """A call of the extension: its refusals come as TmxError, like the library's own.  That memory for a result has run out,
+    or an error of the device, is no refusal: it stays what it is."""
     try:
         return op(*args)
+    except (torch.OutOfMemoryError, torch.AcceleratorError):
+        raise
     except (RuntimeError, NotImplementedError, TypeError) as e:
         raise _lib.TmxError(-1, str(e)) from None
 
