@@ -71,6 +71,22 @@ def test_which_errors_are_refusals(monkeypatch, error, comes_as):
         assert type(e.value) is comes_as
 
 
+@pytest.mark.parametrize("big", [(1 << 32) + 16, (1 << 31) + 16])
+def test_the_ctypes_binding_refuses_numbers_past_32_bits(monkeypatch, big):
+    """It would cut them down to others: a page size of 2^32 + 16 to 16."""
+    monkeypatch.setattr(ops, "_BINDING", "ctypes")
+    monkeypatch.setattr(ops, "_require_gpu", lambda t, name: None)
+    t, c = torch.zeros(1, 2, dtype=torch.int32), [torch.zeros(4, 32, dtype=torch.uint8)]
+    lens = t[0, :1]
+    for call in (lambda: ops.free_pages(t, lens, 8, big), lambda: ops.free_pages(t, lens, big, 16), lambda: ops.fork_pages(c, t, lens, lens, lens, big),
+                 lambda: ops.compact_pages(c, t, lens, big)):
+        with pytest.raises(RuntimeError, match="page_size"):
+            call()
+    k = torch.zeros(ops.fp4_cache_shape(2, 16, 1, 64), dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="max_seq_len"):
+        ops.gather_dequant_kv_fp4(k, k, t, lens, lens, 4, big, torch.bfloat16)
+
+
 @gpu
 def test_modes_and_profilers_see_the_calls():
     want = all_four(*inputs())

@@ -906,6 +906,8 @@ def gather_dequant_kv_fp4(key_cache: torch.Tensor, value_cache: torch.Tensor, bl
         raise RuntimeError("seq_lens and cu_seqlens_k must be contiguous int32, block_table must cover the batch")
     if out_dtype not in (torch.bfloat16, torch.float16):
         raise RuntimeError("rows are read back as bfloat16 or float16")
+    if not 0 <= max_seq_len <= 0x7fffffff:
+        raise RuntimeError(f"bad max_seq_len {max_seq_len}")
     hkv = key_cache.shape[2]
     if out is None:
         k_rows = torch.empty((max(total_rows, 1), hkv, d), dtype=out_dtype, device=dev)
@@ -1024,6 +1026,12 @@ def _page_table(block_table: torch.Tensor, seq_lens: torch.Tensor) -> torch.devi
     return block_table.device
 
 
+def _page_numbers(page_size: int, num_pages: int = 0) -> None:
+    """What the library takes as 32-bit numbers (ctypes would cut larger ones down to others)."""
+    if not 0 < page_size <= 1 << 30 or not 0 <= num_pages <= 1 << 30:
+        raise RuntimeError(f"bad page_size {page_size} or number of pages {num_pages}")
+
+
 def _page_ints(t: torch.Tensor, n: int, name: str) -> None:
     if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() < n:
         raise RuntimeError(f"{name} must be contiguous int32 with an entry per row")
@@ -1057,8 +1065,7 @@ def free_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, num_pages: int
     if C is not None:
         return _page_call(C, "free_pages", block_table, seq_lens, int(num_pages), int(page_size))
     dev = _page_table(block_table, seq_lens)
-    if num_pages < 0:
-        raise RuntimeError("num_pages must not be negative")
+    _page_numbers(page_size, num_pages)
     rows, cols = seq_lens.numel(), block_table.shape[1]
     lib = _lib.load()
     work = lib.tmx_pages_work_ints(rows, cols, num_pages)
@@ -1082,6 +1089,7 @@ def fork_pages(caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq_le
         return _page_call(C, "fork_pages", caches, block_table, seq_lens, parents, fresh, int(page_size))
     dev = _page_table(block_table, seq_lens)
     at, size, stride, pages = _page_list(caches, dev)
+    _page_numbers(page_size, pages)
     _on(dev, (parents, "parents"), (fresh, "fresh"))
     n = parents.numel()
     _page_ints(parents, n, "parents")
@@ -1107,6 +1115,7 @@ def compact_pages(caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq
     if not len(caches):
         raise RuntimeError("compact_pages needs the caches (their first dimension is the pool)")
     at, size, stride, pages = _page_list(caches, dev)
+    _page_numbers(page_size, pages)
     rows, cols = seq_lens.numel(), block_table.shape[1]
     lib = _lib.load()
     work, moves = lib.tmx_pages_work_ints(rows, cols, pages), pages // 2 + 1
