@@ -176,6 +176,10 @@ def test_the_runner_is_asked_for_decode_requests_first():
     assert builder_for("cpu").reorder_batch_threshold is None and B.get_builder_cls().reorder_batch_threshold is None
 
 
+def test_copies_without_layers_are_nothing():
+    assert B.copy_blocks([], torch.tensor([[1, 2]])) is None
+
+
 @gpu
 @pytest.mark.parametrize("dtype, D, H, Hkv", [(torch.bfloat16, 128, 8, 2), (torch.float16, 64, 4, 2)])
 @pytest.mark.parametrize("use_triangle", [True, False])

@@ -423,8 +423,9 @@ class TriangleMixAttentionBackend(_BackendBase):
     def copy_blocks(kv_caches: List[torch.Tensor], src_to_dists: torch.Tensor) -> None:
         """Pages ``src_to_dists[:, 0]`` of every layer's cache ``[2, num_blocks, ...]`` to pages ``src_to_dists[:, 1]``
         (the reference's csrc/cache_kernels.cu copy_blocks), K and V of all layers in one launch."""
-        ops.copy_pages([kv for cache in kv_caches for kv in cache.unbind(0)],
-                       src_to_dists.to(kv_caches[0].device).contiguous() if len(kv_caches) else src_to_dists)
+        if len(kv_caches) == 0:
+            return
+        ops.copy_pages([kv for cache in kv_caches for kv in cache.unbind(0)], src_to_dists.to(kv_caches[0].device).contiguous())
 
     @staticmethod
     def use_cascade_attention(*args, **kwargs) -> bool:
