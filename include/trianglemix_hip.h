@@ -570,7 +570,10 @@ int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* args, void* stream);
  * `caches` the host array of the K and V caches of all layers (same sizes, num_pages pages each).  Which pages are in use
  * follows from block_table [rows, cols] (int32, its rows block_table_stride apart) and seq_lens [rows]: row r holds its
  * first ceil(seq_lens[r] / page_size) entries; a sequence is freed by a length of 0.  Entries that are no page numbers
- * are passed over.  All lists are ascending or in a fixed order, never that of the workgroups.
+ * are passed over.  Nothing else counts: pages held by something that is no row of this table (a prefix cache, a request
+ * outside the batch, a page that stands for none) are free to these calls, and tmx_plan_compaction moves others onto them,
+ * unless a row of their own lists them with a length of so many pages.  Whoever keeps page numbers elsewhere takes the new
+ * ones from new_table.  All lists are ascending or in a fixed order, never that of the workgroups.
  *
  * tmx_free_pages: free_out [num_pages] = the pages no row holds, ascending, -1 behind them; count_out[0] of them.
  * tmx_plan_compaction: of the U pages in use, the k-th one at or past U is to go to the k-th free page before U:

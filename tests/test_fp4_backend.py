@@ -176,6 +176,23 @@ def test_the_runner_is_asked_for_decode_requests_first():
     assert builder_for("cpu").reorder_batch_threshold is None and B.get_builder_cls().reorder_batch_threshold is None
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_cache_made_from_a_spec(D):
+    """The way from a spec to the tensor that a runner takes (gpu_model_runner.py: bytes from the spec, blocks from the memory
+    at hand, a raw tensor viewed as the backend's shape)."""
+    spec = types.SimpleNamespace(block_size=32, num_kv_heads=8, head_size=D, dtype=torch.uint8,
+                                 page_size_bytes=2 * 32 * 8 * (D // 2 + D // 32))
+    raw = torch.zeros(11 * spec.page_size_bytes, dtype=torch.int8)
+    assert raw.numel() % spec.page_size_bytes == 0
+    shape = B.get_kv_cache_shape(raw.numel() // spec.page_size_bytes, spec.block_size, spec.num_kv_heads, spec.head_size, "mxfp4")
+    cache = raw.view(spec.dtype).view(shape)
+    k, v = cache.unbind(0)
+    assert k.shape == ops.fp4_cache_shape(11, 32, 8, D) and k.stride(0) == v.stride(0) == spec.page_size_bytes // 2
+    for bad in ((11, 32, 8, D // 2 + D // 32), (11, 48, 8, D)):
+        with pytest.raises((RuntimeError, ValueError)):
+            B.get_kv_cache_shape(*bad, "mxfp4")
+
+
 def test_copies_without_layers_are_nothing():
     assert B.copy_blocks([], torch.tensor([[1, 2]])) is None
 

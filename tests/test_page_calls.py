@@ -135,3 +135,29 @@ def test_plain_calls_stay_plain():
         assert m.copy_pages(caches, torch.tensor([[9, 5]], device=DEV)) is None
     with torch.no_grad():
         assert m.compact_pages(caches, table, lens, 16) is not NotImplemented
+
+
+@gpu
+def test_pages_held_by_no_sequence_are_kept_by_a_row_of_their_own():
+    """The null page 0, two blocks of a prefix cache and a request outside the batch: a row each, of whole pages."""
+    page, pages = 16, 40
+    table = torch.full((6, 4), -1, dtype=torch.int32)
+    table[0, 0] = 0
+    table[1, :2] = torch.tensor([33, 12])
+    table[2, :3] = torch.tensor([39, 5, 20])
+    table[3, :3], table[4, :2] = torch.tensor([33, 38, 7]), torch.tensor([30, 31])  # two sequences, one that shares page 33
+    table[5, :4] = torch.tensor([1, 2, 3, 4])  # ended
+    lens = torch.tensor([page, 2 * page, 3 * page, 37, 17, 0], dtype=torch.int32)
+    start = [torch.randint(0, 256, (pages, 64), dtype=torch.uint8) for _ in range(2)]
+    caches = [x.to(DEV) for x in start]
+    t, n = table.to(DEV), lens.to(DEV)
+    held = {0, 33, 12, 39, 5, 20, 38, 7, 30, 31}
+    free, count = ops.free_pages(t, n, pages, page)
+    assert set(free[:int(count)].tolist()) == set(range(pages)) - held
+    new, used = ops.compact_pages(caches, t, n, page)
+    assert int(used) == len(held) and int(new[0, 0]) == 0 and new[5].tolist() == [-1] * 4
+    for r in range(5):
+        for c in range(-(-int(lens[r]) // page)):
+            for x, y in zip(start, caches):
+                assert torch.equal(y[int(new[r, c])].cpu(), x[int(table[r, c])])
+    assert int(new[1, 0]) == int(new[3, 0])

@@ -1059,7 +1059,9 @@ def copy_pages(caches: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
 def free_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, num_pages: int, page_size: int):
     """The pages of a pool of ``num_pages`` that no sequence uses: ``(ids, count)``, int32 ``[num_pages]`` ascending with -1
     behind the last, and ``[1]``.  Row ``r`` of ``block_table`` uses its first ``ceil(seq_lens[r] / page_size)`` entries; a
-    sequence is freed by a length of 0.  Nothing is read back to the host."""
+    sequence is freed by a length of 0.  Only these rows count: a page held otherwise -- by a prefix cache, a request outside
+    the batch, a page that stands for none -- needs a row of its own that lists it, with a length to match (pages x
+    ``page_size``), here and in :func:`compact_pages`.  Nothing is read back to the host."""
     _require_gpu(block_table, "block_table")
     C = _module()
     if C is not None:
@@ -1082,7 +1084,8 @@ def fork_pages(caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq_le
     max_blocks]`` table shares the full pages of row ``parents[i]``; the parent's partial last page, if it has one, is
     copied to page ``fresh[i]`` in every cache of the list and that page takes its place.  Entries behind are -1; a parent
     that is no row gives a row of -1.  The fresh pages (:func:`free_pages`) are distinct and not in use; one whose parent
-    ends on a page boundary stays free."""
+    ends on a page boundary stays free.  Where the pool has run short :func:`free_pages` gives -1, and so does the child's row:
+    its keys there count as NaN."""
     _require_gpu(block_table, "block_table")
     C = _module()
     if C is not None:
@@ -1106,7 +1109,9 @@ def compact_pages(caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq
     """Closes a pool up: afterwards its ``U`` pages in use are the pages 0 .. U - 1.  Of the pages in use the k-th one at or
     past U moves to the k-th free page before it, in every cache of the list.  Returns ``(table, count)``: the block table
     afterwards (a new int32 ``[rows, max_blocks]``, -1 behind a row's entries) and U (int32 ``[1]``).  Pages shared by
-    several rows move once.  Nothing is read back to the host."""
+    several rows move once.  Every page that no row lists is taken for free and may be written over (:func:`free_pages`: a
+    row for pages held otherwise), and whoever keeps page numbers elsewhere has to take them from the new table; pages 0 ..
+    n - 1 that a row lists stay where they are.  Nothing is read back to the host."""
     _require_gpu(block_table, "block_table")
     C = _module()
     if C is not None:
