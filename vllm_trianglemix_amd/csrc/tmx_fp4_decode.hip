@@ -136,15 +136,17 @@ __device__ __forceinline__ int fp4_len_of(const Fp4DecodeParams& p, const Fp4Pla
   return plan.per == 1 ? __builtin_amdgcn_readlane(plan.len, b) : fp4_len(p, fp4_sload(p.seq_lens + b));
 }
 
-// Workgroups resident per CU.  Two per CU with a tile read ahead per wave have 70 KB in flight, all that the memory
-// system takes (whole calls on inputs that no cache holds, head size 128: 64 x 8192 tokens 92.2 us with two, 99.1 with three, 95.4
+// Workgroups resident per CU.  Two per CU with a tile read ahead per wave have 70 KB in flight at head size 128, all that the
+// memory system takes (whole calls on inputs that no cache holds: 64 x 8192 tokens 92.2 us with two, 99.1 with three, 95.4
 // with two that read two tiles ahead; 4 x 16384 21.0 and 22.9 with three; 32 ragged requests 33.2 and 35.2).  Head size 64 has
-// half the bytes per tile (64 x 8192, fp16: 64.4 us with four, 65.9 with two).
-constexpr int fp4_wgs_per_cu(int head_dim, int rows) { return head_dim == 128 || rows > 16 ? 2 : 4; }
+// half the bytes per tile and would leave room for four, but gains nothing by it (bf16, 4 rows per K/V head, two / three /
+// four: 64 x 8192 65 / 65 / 67 us, 32 ragged requests 25.4 / 24.9 / 25.9, 8 x 65536 of one K/V head 17.7 / 17.7 / 19.4; fp16,
+// 16 rows: 67 / 72 / 69, 27.0 / 27.5 / 28.5, 19.3 / 19.4 / 21.7, with registers spilled at four).
+constexpr int kFp4WgsPerCu = 2;
 
 // NT column tiles of 16 rows; HALF: one tile, at most 8 rows, columns 8..15 carry the probabilities' second terms
 template <int D, bool BF16, int NT, bool HALF>
-__global__ __launch_bounds__(256, fp4_wgs_per_cu(D, 16 * NT)) void fp4_decode_kernel(const Fp4DecodeParams p) {
+__global__ __launch_bounds__(256, kFp4WgsPerCu) void fp4_decode_kernel(const Fp4DecodeParams p) {
   static_assert(!HALF || NT == 1, "the half form has one tile");
   constexpr int DT = D / 16;        // row tiles of the second product
   constexpr int VW = D / 32;        // words of V codes per lane and page-half
@@ -653,8 +655,8 @@ __global__ __launch_bounds__(D / 4 * PIECES < 256 ? 256 : D / 4 * PIECES) void f
 
 // Spans per unit: as many as there are workgroups resident together on the chip.
 static int fp4_row_groups(int64_t rows) { return (int)((rows + 31) / 32); }
-static int fp4_spans(int head_dim, int64_t rows, int kv_heads, int cus) {
-  return imax(1, cus * fp4_wgs_per_cu(head_dim, rows > 16 ? 32 : 16) / (kv_heads * fp4_row_groups(rows)));
+static int fp4_spans(int64_t rows, int kv_heads, int cus) {
+  return imax(1, cus * kFp4WgsPerCu / (kv_heads * fp4_row_groups(rows)));
 }
 
 static int fp4_cus(int* out) {
@@ -699,7 +701,7 @@ extern "C" int64_t tmx_decode_fp4_workspace_rows(int batch, int rows_per_request
   if (batch <= 0 || rows_per_request <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0) return 0;
   if (num_cus <= 0 && fp4_cus(&num_cus) != TMX_OK) return -1;
   const int64_t R = (int64_t)rows_per_request * (num_heads / num_kv_heads);
-  return (fp4_spans(head_dim, R > 64 ? 64 : R, num_kv_heads, num_cus) + (int64_t)batch) * rows_per_request * num_heads + batch;
+  return (fp4_spans(R > 64 ? 64 : R, num_kv_heads, num_cus) + (int64_t)batch) * rows_per_request * num_heads + batch;
 }
 
 extern "C" int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* a, void* stream) {
@@ -750,7 +752,7 @@ extern "C" int tmx_decode_attention_fp4(const tmx_decode_fp4_args_t* a, void* st
     if (rc != TMX_OK) return rc;
   }
   Fp4DecodeParams p{};
-  p.spans = fp4_spans(a->head_dim, R, a->num_kv_heads, cus);
+  p.spans = fp4_spans(R, a->num_kv_heads, cus);
   p.row_groups = fp4_row_groups(R);
   p.units = a->num_kv_heads * p.row_groups;
   const int64_t rows = (p.spans + (int64_t)a->batch) * a->rows_per_request * a->num_heads;
