@@ -523,7 +523,9 @@ int tmx_gather_dequant_kv_fp8(const void* key_cache, const void* value_cache, in
  * these rows through tmx_attention in its contiguous mode.
  * tmx_decode_attention_fp4: rows_per_request = m query rows per request, [batch * m, num_heads, head_dim]; row b m + j sits
  * at position seq_lens[b] - m + j and attends to the keys up to its position (the keys of the step are in the cache
- * already).  m = 1 is a decode step, m > 1 checks drafted tokens; m * num_heads / num_kv_heads <= 64.  seq_lens[b] <= 0
+ * already).  m = 1 is a decode step, m > 1 checks drafted tokens; m * num_heads / num_kv_heads <= 64.  Scores are held in
+ * fp32 (q k, and q k scale log2(e), below 3e38 in magnitude), sums of p |v| in fp32 before the division, with p up to 2^8 (|v| below 2^119 /
+ * keys is always finite).  out must not overlap q.  seq_lens[b] <= 0
  * marks padding, its out rows are left alone, as are rows at negative positions.  As in tmx_decode_attention the launch
  * depends on the batch size alone (it replays under a graph) and the work area -- partial_o [rows][head_dim], partial_ml
  * [rows][2], rows = tmx_decode_fp4_workspace_rows(...), whatever they hold -- belongs to one call at a time.

@@ -4,8 +4,10 @@
 // lines, early, and keep the vector units out of their way.
 //
 //   workgroup = 4 waves = a span of 32-key tiles x one K/V head; the waves take the span's tiles in turn and meet only at
-//   a request's end.  Rows = rows_per_request x (query heads per K/V head), all of them columns of the same products, so
-//   a head's K/V are read once whatever the group size.
+//   a request's end.  Rows = rows_per_request x (query heads per K/V head), up to 32 of them columns of the same products, so
+//   a head's K/V are read and converted once for them whatever the group size.  33 to 64 rows are two groups, each with
+//   workgroups of its own that read and convert K/V again (16 x 2878 .. 4111 tokens, 64 / 8 heads, bf16, 1 / 2 / 4 / 8 rows per
+//   request, i.e. 8 to 64 per K/V head: 19.8 / 21.5 / 30.9 / 43.0 us).
 //   Scores S^T = K Q^T (v_mfma_f32_16x16x32_bf16, D / 32 of them per 16 keys): lane (m = lane % 16, g = lane / 16) holds
 //   columns [g D/4, (g + 1) D/4) of key row m, one load and one scale; the codes become bf16, which is exact (one fraction
 //   bit, power-of-two scales).  The head dimension may be summed in any order as long as Q^T is laid out alike.  fp16
@@ -19,7 +21,8 @@
 //   Probabilities are held as two bf16 terms (16 significant bits; one term alone would cost as much accuracy as the
 //   rounding of the output).  Up to 8 rows, columns 8..15 repeat the rows and carry the second term: no extra product.
 //   Their sum is one more product, with ones.
-//   Every load instruction of the loop reads one contiguous run of a page-half (1 KB of codes) from a scalar base.
+//   Every load instruction of the loop reads one contiguous run of a page-half (16 keys: 1 KB of codes, 512 bytes at head
+//   size 64) from a scalar base.
 //   The running maximum is raised only when a score exceeds it by more than 2^kSlack (factors stay below 2^8 in fp32).
 #include <atomic>
 #include <type_traits>
@@ -681,7 +684,8 @@ static void fp4_launch(const Fp4DecodeParams& p, hipStream_t s) {
   else fp4_decode_kernel<D, BF16, 2, false><<<grid, 256, 0, s>>>(p);
   // Pieces of a row that are joined side by side, by how many an average request can have (four more of each are in
   // flight), with 2 / 8 / 32 of them: 16 x 4 drafted rows of up to 5 pieces 4.7 / 5.2 / 16.7 us, 8 requests of 64 pieces 6.1 /
-  // 4.6 / 4.6, one of 512 pieces 22.9 / 8.2 / 6.0.
+  // 4.6 / 4.6, one of 512 pieces 22.9 / 8.2 / 6.0.  (One request with nearly all pieces beside many short ones is joined as
+  // the average would be: the whole call for 131072 tokens of one K/V head takes 16.3 us, beside 64 requests of 64 32.2.)
   const unsigned rows = (unsigned)(p.m * p.H);
   const int pieces = p.spans / p.batch;
   auto join = [&](auto pieces_) {

@@ -948,7 +948,8 @@ def decode_attention_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out:
     (``reshape_and_cache_fp4``).  One row is a decode step, several check drafted tokens (at most 64 rows per K/V head:
     ``rows_per_request * H / Hkv <= 64``).  The launch depends on the batch size only: it can be captured and replayed
     after ``seq_lens`` / ``block_table`` / the caches changed in place.  ``seq_lens[b] <= 0`` marks a padding request; its
-    rows of ``out``, and rows at negative positions, are left alone.  Keys whose page does not exist count as NaN.
+    rows of ``out``, and rows at negative positions, are left alone.  ``out`` must not overlap ``q``.  Keys whose page does not
+    exist count as NaN.
     ``workspace``: :func:`decode_fp4_workspace`."""
     if workspace is None or len(workspace) < 2 or workspace[0] is None or workspace[1] is None:
         raise RuntimeError("decode_attention_fp4 needs its work area (ops.decode_fp4_workspace for the batch size)")
