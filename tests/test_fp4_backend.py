@@ -213,7 +213,8 @@ def test_mixed_steps_against_the_formula(monkeypatch, dtype, D, H, Hkv, use_tria
             ([1, 1, 40], [300, 17, 40], None, (2, 1)), ([1, 1, 1, 100, 3], [33, 500, 1, 180, 90], None, (3, 1)),
             ([3, 3, 70, 1], [200, 3, 150, 64], None, (2, 3)), ([1, 80, 1], [129, 200, 90], [100, 400, 90], (1, 1)),
             ([2, 2, 50], [120, 70, 90], [200, 70, 90], (0, 0) if use_triangle else (2, 2)), ([50, 1, 1], [60, 200, 300], None, (0, 0)),
-            ([1, 1, 1, 17], [1, 2, 3, 17], None, (3, 1))):
+            ([1, 1, 1, 17], [1, 2, 3, 17], None, (3, 1)), ([3, 3, 1, 1, 1], [80, 300, 65, 1, 400], None, (2, 3)),
+            ([1] * 20 + [2, 2], list(range(3, 23)) + [200, 9], None, (20, 1))):
         T, R = sum(q_lens), len(q_lens)
         width = max(-(-n // page) for n in seq_lens)
         table = rng.permutation(R * width).astype(np.int32).reshape(R, width)
